@@ -12,6 +12,8 @@ std::vector<at::Tensor> add_rmsnorm_fwd(at::Tensor x, at::Tensor delta, at::Tens
 std::vector<at::Tensor> rmsnorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor rstd);
 std::vector<at::Tensor> rmsnorm_bwd_add(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor rstd,
                                         c10::optional<at::Tensor> ds);
+std::vector<at::Tensor> rmsnorm_fp8(at::Tensor x, c10::optional<at::Tensor> delta, at::Tensor w, double eps, bool pow2,
+                                    bool mn_major);
 // elementwise.cu
 at::Tensor rope_qkv(at::Tensor qkv, at::Tensor positions, at::Tensor cache, int64_t nq, int64_t nkv, int64_t hd,
                     bool inverse);
@@ -44,6 +46,15 @@ std::vector<at::Tensor> flash_attn_bwd(at::Tensor dout, at::Tensor q, at::Tensor
                                        bool causal);
 at::Tensor paged_decode_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor block_tables,
                              at::Tensor seq_lens, double scale, int64_t max_seq_len, double k_scale, double v_scale);
+// cache_pages.cu
+std::tuple<int64_t, int64_t> copy_cache_pages(at::Tensor cache, std::vector<int64_t> src, std::vector<int64_t> dst,
+                                              std::vector<int64_t> tokens);
+// shared_prefix_attn.cu
+at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, at::Tensor seq_lens, int64_t nq,
+                              int64_t nkv);
+at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor block_tables,
+                              at::Tensor plan, int64_t groups, double scale, double k_scale, double v_scale);
+int64_t shared_prefix_error_flag(bool reset);
 // gemm_tcgen05.cu
 at::Tensor gemm_nt(at::Tensor a, at::Tensor b);
 int64_t gemm_error_flag(bool reset);
@@ -158,6 +169,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm_bwd", &rmsnorm_bwd);
   m.def("rmsnorm_bwd_add", &rmsnorm_bwd_add, py::arg("dy"), py::arg("x"), py::arg("w"), py::arg("rstd"),
         py::arg("ds") = py::none());
+  m.def("rmsnorm_fp8", &rmsnorm_fp8, py::arg("x"), py::arg("delta"), py::arg("w"), py::arg("eps"), py::arg("pow2"),
+        py::arg("mn_major"), "RMSNorm of x (+ delta) with an e4m3 output, one scale per 128 values");
   m.def("rope_qkv", &rope_qkv);
   m.def("swiglu_fwd", &swiglu_fwd);
   m.def("swiglu_bwd", &swiglu_bwd);
@@ -175,6 +188,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("flash_attn_fwd", &flash_attn_fwd);
   m.def("flash_attn_bwd", &flash_attn_bwd);
   m.def("paged_decode_attn", &paged_decode_attn);
+  m.def("copy_cache_pages", &copy_cache_pages, "copies of KV-cache pages in every layer, page lists on the host");
+  m.def("shared_prefix_plan", &shared_prefix_plan, "work plan of shared_prefix_attn for one decode step");
+  m.def("shared_prefix_attn", &shared_prefix_attn, "paged decode attention, the prefix of a group read once");
+  m.def("shared_prefix_error_flag", &shared_prefix_error_flag, py::arg("reset") = false,
+        "error word: 1 group bounds, 2 block-table entry outside the cache, 3 expired wait");
   m.def("gemm_nt", &gemm_nt);
   m.def("gemm_error_flag", &gemm_error_flag, py::arg("reset") = false);
   m.def("gemm_rs", &gemm_rs);

@@ -7,7 +7,11 @@
 // vector accesses.  The backward accumulates the weight gradient per warp in
 // shared memory and writes one fp32 partial row per CTA; a second kernel sums
 // the partials (deterministic, no atomics).
-#include "common.cuh"
+//
+// rmsnorm_fp8 is the forward whose output goes to a block-scaled fp8 projection:
+// it leaves the normalised row as e4m3 with one scale per 128 values (see the
+// kernel's comment).
+#include "fp8_scale.cuh"
 
 #include <cstdlib>
 
@@ -126,6 +130,113 @@ rmsnorm_fwd_rowcta_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[k][i] = v[k][i] * r * g[i];
       yr[j] = pack8(v[k]);
+    }
+  }
+}
+
+// RMSNorm (of x + delta) with an e4m3 output, one scale per 128 values of a row:
+//
+//   s = x + delta (rounded to T, stored);  y = s * rsqrt(mean(s^2) + eps) * w (rounded to T)
+//   scale = max|y| / 448 over 128 values (or the next power of two);  q = e4m3(y / scale)
+//
+// One pass over memory: 2 B of x, 2 of delta, 2 of s and 1 of q per value (bf16),
+// where the separate norm and quantisation move 11.  The row stays in
+// registers (packed, NV vectors of 8 per thread) between the sum of squares and
+// the output, so its loads are all in flight at once; 16 neighbouring lanes hold
+// the 128 values of a scale, so the maximum is a half-warp shuffle.
+//
+// y is rounded to T before it is quantised, and TPR threads take a row's vectors
+// in the order of the unquantised kernels above: the result equals rmsnorm_fwd /
+// add_rmsnorm_fwd followed by quant_fp8_group(_t) bit for bit (a NaN stays one).
+// TPR = 128 is the few-row (decode) kernel, TPR = 32 the many-row one, by the same
+// rule.
+//
+// Scales are row-major [rows, H/128], or (mn_major) [H/128, ld] with the padding
+// rows up to ld set to 1, the layout that the hardware-scaled GEMM reads.
+template <typename T>
+struct alignas(8 * sizeof(T)) Vec8 {
+  T v[8];
+};
+
+template <typename T, int NV, int TPR>
+__global__ void __launch_bounds__(128)
+rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* __restrict__ w,
+                   T* __restrict__ s_out, __nv_fp8_e4m3* __restrict__ q, float* __restrict__ scales, int rows, int H,
+                   float eps, bool pow2, int ld) {
+  pdl_launch_dependents();
+  __shared__ float red[32];
+  const int t = TPR == 128 ? threadIdx.x : (threadIdx.x & 31);
+  const int row = TPR == 128 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int ngroups = H / 128;
+  if (row >= rows) {  // padding rows of the mn-major scales (ld is 0 otherwise); uniform over a row's threads
+    if (row < ld)
+      for (int g = t; g < ngroups; g += TPR) scales[(size_t)g * ld + row] = 1.f;
+    return;
+  }
+  const int nv = H / 8;
+  const Vec8<T>* xr = reinterpret_cast<const Vec8<T>*>(x + (size_t)row * H);
+  const Vec8<T>* dr = delta ? reinterpret_cast<const Vec8<T>*>(delta + (size_t)row * H) : nullptr;
+  Vec8<T>* sr = s_out ? reinterpret_cast<Vec8<T>*>(s_out + (size_t)row * H) : nullptr;
+  const Vec8<T>* wr = reinterpret_cast<const Vec8<T>*>(w);
+  Vec8<T> f[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int j = t + k * TPR;
+    if (j < nv) f[k] = xr[j];
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int j = t + k * TPR;
+    if (j < nv) {
+      if (dr) {
+        const Vec8<T> d = dr[j];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[k].v[i] = from_f<T>(to_f(f[k].v[i]) + to_f(d.v[i]));
+        sr[j] = f[k];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = to_f(f[k].v[i]);
+        ss += v * v;
+      }
+    }
+  }
+  ss = TPR == 128 ? block_sum(ss, red) : warp_sum(ss);
+  const float r = rsqrtf(ss / H + eps);
+  uint2* qr = reinterpret_cast<uint2*>(q + (size_t)row * H);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int j = t + k * TPR;
+    float y[8], amax = 0.f;
+    if (j < nv) {
+      const Vec8<T> g = wr[j];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = to_f(from_f<T>(to_f(f[k].v[i]) * r * to_f(g.v[i])));
+        amax = fmaxf(amax, fabsf(y[i]));
+      }
+    }
+    // H % 128 == 0: a half-warp's 16 vectors are all inside the row or all outside
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (j < nv) {
+      const float sc = fp8_scale(amax, pow2);
+      const float inv = 1.f / sc;
+      uint32_t p[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h] * inv, y[4 * h + 1] * inv), __NV_SATFINITE,
+                                                     __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h + 2] * inv, y[4 * h + 3] * inv),
+                                                     __NV_SATFINITE, __NV_E4M3);
+        p[h] = lo | (hi << 16);
+      }
+      qr[j] = make_uint2(p[0], p[1]);
+      if ((t & 15) == 0) {
+        const int g = j >> 4;
+        scales[ld ? (size_t)g * ld + row : (size_t)row * ngroups + g] = sc;
+      }
     }
   }
 }
@@ -272,6 +383,62 @@ std::vector<at::Tensor> add_rmsnorm_fwd(at::Tensor x, at::Tensor delta, at::Tens
   });
   RLB_CUDA_CHECK(cudaGetLastError());
   return {y, s, rstd};
+}
+
+// (q [rows, H] e4m3, scales fp32 [rows, H/128] or, mn_major, [H/128, rows rounded up to 128],
+//  s = x + delta when delta is given)
+std::vector<at::Tensor> rmsnorm_fp8(at::Tensor x, c10::optional<at::Tensor> delta, at::Tensor w, double eps, bool pow2,
+                                    bool mn_major) {
+  check_rows(x, w);
+  RLB_CHECK(w.is_cuda() && w.device() == x.device() && w.is_contiguous(), "rmsnorm_fp8: weight on another device");
+  const bool add = delta.has_value() && delta->defined();
+  if (add)
+    RLB_CHECK(delta->sizes() == x.sizes() && delta->is_contiguous() && delta->scalar_type() == x.scalar_type() &&
+                  delta->device() == x.device(),
+              "rmsnorm_fp8: delta must match the input");
+  const int H = x.size(1);
+  RLB_CHECK(H % 128 == 0 && H >= 128 && H <= 16384, "rmsnorm_fp8: hidden size must be a multiple of 128, at most 16384");
+  RLB_CHECK(x.size(0) <= 0x7fffff00LL, "rmsnorm_fp8: too many rows");
+  const int64_t align = 8 * x.element_size();
+  for (const at::Tensor& t : {x, w, add ? *delta : x})
+    RLB_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % align == 0, "rmsnorm_fp8: tensors must be aligned to 8 values");
+  const c10::cuda::CUDAGuard g(x.device());
+  const int rows = x.size(0);
+  const int ld = mn_major ? std::max(128, (rows + 127) / 128 * 128) : 0;
+  auto f32 = x.options().dtype(at::kFloat);
+  auto q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  auto scales = mn_major ? at::empty({H / 128, ld}, f32) : at::empty({rows, H / 128}, f32);
+  at::Tensor s;
+  std::vector<at::Tensor> out{q, scales};
+  if (add) out.push_back(s = at::empty_like(x));
+  const int out_rows = std::max(rows, ld);
+  if (out_rows == 0) return out;
+  // 128 threads a row while the rows are few, a warp a row when there are enough of them: the
+  // rule of rmsnorm_fwd, whose sums it repeats.  Rows beyond 8192 values always take 128 threads.
+  const bool cta = H > 8192 || use_rowcta(x, H, rows);
+  RLB_DISPATCH_FLOAT(x.scalar_type(), "rmsnorm_fp8", [&] {
+    auto launch = [&](auto nv, auto tpr) {
+      constexpr int NV = decltype(nv)::value, TPR = decltype(tpr)::value;
+      rmsnorm_fp8_kernel<scalar_t, NV, TPR><<<TPR == 128 ? out_rows : (out_rows + 3) / 4, 128, 0, stream()>>>(
+          (const scalar_t*)x.data_ptr(), add ? (const scalar_t*)delta->data_ptr() : nullptr,
+          (const scalar_t*)w.data_ptr(), add ? (scalar_t*)s.data_ptr() : nullptr, (__nv_fp8_e4m3*)q.data_ptr(),
+          scales.data_ptr<float>(), rows, H, (float)eps, pow2, ld);
+    };
+    using std::integral_constant;
+    if (cta) {
+      integral_constant<int, 128> tpr;
+      if (H <= 4096) launch(integral_constant<int, 4>{}, tpr);
+      else if (H <= 8192) launch(integral_constant<int, 8>{}, tpr);
+      else launch(integral_constant<int, 16>{}, tpr);
+    } else {
+      integral_constant<int, 32> tpr;
+      if (H <= 2048) launch(integral_constant<int, 8>{}, tpr);
+      else if (H <= 4096) launch(integral_constant<int, 16>{}, tpr);
+      else launch(integral_constant<int, 32>{}, tpr);
+    }
+  });
+  RLB_CUDA_CHECK(cudaGetLastError());
+  return out;
 }
 
 static std::vector<at::Tensor> rmsnorm_bwd_impl(at::Tensor dy, at::Tensor x, at::Tensor w, at::Tensor rstd,

@@ -585,6 +585,25 @@ class TransformerLM(nn.Module):
             return fp8_linear_mx(x, q, sc) if self.fp8_pow2 else fp8_linear(x, q, sc)
         return linear(x, self._params[name])
 
+    def _norm_lin_infer(self, x: torch.Tensor, delta: Optional[torch.Tensor], norm: str, name: str, project):
+        """Rollout: RMSNorm of ``x`` (``+ delta``) and the projection ``name`` that reads it;
+        returns (projection, residual stream).  With fp8 weights for ``name`` the norm quantises
+        its output itself (the same values as norm, then quantisation inside ``project``)."""
+        w, eps, fw = self._params[norm], self.cfg.rms_eps, self.fp8_weights
+        if (fw is not None and self._in_rollout and self.lora is None and name in fw and x.dtype == torch.bfloat16
+                and x.shape[-1] % 128 == 0 and x.shape[-1] <= 8192):
+            from rl_b200.ops.fp8_gemm import fp8_linear_quantised
+            from rl_b200.ops.norm import add_rms_norm_fp8, rms_norm_fp8
+
+            mx = self.fp8_pow2
+            if delta is None:
+                (h, sc), s = rms_norm_fp8(x, w, eps, mx), x
+            else:
+                h, sc, s = add_rms_norm_fp8(x, delta, w, eps, mx)
+            return fp8_linear_quantised(h, sc, *fw[name], mx), s
+        h, s = (rms_norm(x, w, eps), x) if delta is None else add_rms_norm(x, delta, w, eps)
+        return project(h, name), s
+
     def _col_linear(self, h: torch.Tensor, name: str) -> torch.Tensor:
         """Column-parallel projection (+ LoRA delta when adapters are attached)."""
         if self._in_rollout and self.fp8_weights is not None and self.lora is None:
@@ -920,19 +939,15 @@ class TransformerLM(nn.Module):
         eps = self.cfg.rms_eps
         for i in range(self.cfg.num_layers):
             p = f"model.layers.{i}."
-            if resid is None:
-                h = rms_norm(x, self._params[p + "input_layernorm.weight"], eps)
-                s = x
-            else:
-                h, s = add_rms_norm(x, resid, self._params[p + "input_layernorm.weight"], eps)
-            qkv = self._qkv(i, h, positions)
+            qkv, s = self._norm_lin_infer(x, resid, p + "input_layernorm.weight", p + "self_attn.qkv_proj.weight",
+                                          self._col_linear)
+            qkv = self._qkv(i, None, positions, qkv)
             q, k, v = self._split_heads(qkv)
             kc, vc = kv.layer(i)
             write_kv_cache(k, v, kc, vc, slot_mapping, *kv.scales(i))
             o, _ = flash_attn_varlen_fwd(q, k, v, cu_seqlens, max_seqlen, causal=True)
             a = self._tp_sum(self._lin_infer(o.reshape(o.shape[0], -1), p + "self_attn.o_proj.weight"))
-            h2, s2 = add_rms_norm(s, a, self._params[p + "post_attention_layernorm.weight"], eps)
-            m = self._mlp_infer(i, h2)
+            m, s2 = self._norm_mlp_infer(i, s, a)
             x, resid = s2, m
             self._capture(i, x, resid)
         h, _ = add_rms_norm(x, resid, self._params["model.norm.weight"], eps)
@@ -977,12 +992,9 @@ class TransformerLM(nn.Module):
         eps = self.cfg.rms_eps
         for i in range(self.cfg.num_layers):
             p = f"model.layers.{i}."
-            if resid is None:
-                h = rms_norm(x, self._params[p + "input_layernorm.weight"], eps)
-                s = x
-            else:
-                h, s = add_rms_norm(x, resid, self._params[p + "input_layernorm.weight"], eps)
-            qkv = self._qkv(i, h, positions)
+            qkv, s = self._norm_lin_infer(x, resid, p + "input_layernorm.weight", p + "self_attn.qkv_proj.weight",
+                                          self._col_linear)
+            qkv = self._qkv(i, None, positions, qkv)
             q, k, v = self._split_heads(qkv)
             kc, vc = kv.layer(i)
             ks, vs = kv.scales(i)
@@ -990,8 +1002,7 @@ class TransformerLM(nn.Module):
             o = paged_decode_attention(q, kc, vc, block_tables, seq_lens, max_seq_len=max_seq_len,
                                        k_scale=ks, v_scale=vs)
             a = self._tp_sum(self._lin_infer(o.reshape(o.shape[0], -1), p + "self_attn.o_proj.weight"))
-            h2, s2 = add_rms_norm(s, a, self._params[p + "post_attention_layernorm.weight"], eps)
-            m = self._mlp_infer(i, h2)
+            m, s2 = self._norm_mlp_infer(i, s, a)
             x, resid = s2, m
             self._capture(i, x, resid)
         h, _ = add_rms_norm(x, resid, self._params["model.norm.weight"], eps)
@@ -1041,17 +1052,20 @@ class TransformerLM(nn.Module):
             dist.all_reduce(x, group=self.ps.tp_group)
         return x
 
-    def _mlp_infer(self, i: int, h: torch.Tensor) -> torch.Tensor:
+    def _norm_mlp_infer(self, i: int, x: torch.Tensor, delta: torch.Tensor):
+        """Rollout MLP sub-layer of the residual stream ``x + delta``: (MLP output, residual stream)."""
         p = f"model.layers.{i}."
         if self.cfg.is_moe:
+            h, s = add_rms_norm(x, delta, self._params[p + "post_attention_layernorm.weight"], self.cfg.rms_eps)
             sp = self.sequence_parallel
             self.sequence_parallel = False
             try:
-                return self._moe_block(i, h)
+                return self._moe_block(i, h), s
             finally:
                 self.sequence_parallel = sp
-        gu = self._lin_infer(h, p + "mlp.gate_up_proj.weight")
-        return self._tp_sum(self._lin_infer(swiglu(gu), p + "mlp.down_proj.weight"))
+        gu, s = self._norm_lin_infer(x, delta, p + "post_attention_layernorm.weight", p + "mlp.gate_up_proj.weight",
+                                     self._lin_infer)
+        return self._tp_sum(self._lin_infer(swiglu(gu), p + "mlp.down_proj.weight")), s
 
     def logits_infer(self, hidden: torch.Tensor) -> torch.Tensor:
         """Full-vocab logits for sampling ``[B, V]`` (TP shards all-gathered)."""

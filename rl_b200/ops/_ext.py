@@ -50,6 +50,8 @@ _KERNELS_PER_CALL = {
     "symm_close": 0,
     "symm_view": 0,
     "moe_router_topk": 3,
+    "shared_prefix_attn": 2,
+    "shared_prefix_error_flag": 0,
     "bounds_errors": 0,
     "dp_error_flag": 0,
     "nvls_error_flag": 0,
@@ -128,7 +130,7 @@ def use_native(*tensors: torch.Tensor) -> bool:
 # every kernel family's device error word (set when a bounded wait runs out)
 ERROR_FLAGS = ("gemm_error_flag", "gemm_sm100_error_flag", "gemm_fp8_error_flag", "grouped_gemm_error_flag",
                "gemm_decode_error_flag", "decode_ar_error_flag", "attn_error_flag", "attn_tc_error_flag",
-               "ep_error_flag", "dp_error_flag", "nvls_error_flag")
+               "ep_error_flag", "dp_error_flag", "nvls_error_flag", "shared_prefix_error_flag")
 
 
 BOUNDS_SITES = {1: "KV-cache slot", 2: "paged-attention block-table entry",

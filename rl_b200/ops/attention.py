@@ -14,13 +14,16 @@ Layouts
 * paged cache: ``k_cache, v_cache [num_blocks, block_size, nkv, hd]``,
   ``block_tables [B, max_blocks] int32``, ``seq_lens [B] int32``;
   ``slot_mapping [T] int64`` = block * block_size + offset for writes.
+* shared prefixes: rows ``[group_starts[g], group_starts[g+1])`` of a decode batch have the same
+  keys in their first ``prefix_lens[g]`` positions (samples of one prompt);
+  ``shared_prefix_decode_attention`` reads those once per group.
 """
 
 from __future__ import annotations
 
 import math
 import os
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -31,6 +34,9 @@ __all__ = [
     "flash_attn_varlen_ref",
     "paged_decode_attention",
     "paged_decode_attention_ref",
+    "SharedPrefixPlan",
+    "shared_prefix_plan",
+    "shared_prefix_decode_attention",
     "write_kv_cache",
     "write_kv_cache_ref",
 ]
@@ -219,3 +225,82 @@ def paged_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, scale: O
         k_cache = k_cache.to(torch.float32) * k_scale
         v_cache = v_cache.to(torch.float32) * v_scale
     return paged_decode_attention_ref(q, k_cache, v_cache, block_tables, seq_lens, scale)
+
+
+class SharedPrefixPlan(NamedTuple):
+    """Work plan of :func:`shared_prefix_decode_attention` for one set of lengths."""
+
+    buf: torch.Tensor
+    rows: int
+    groups: int
+    heads: int
+    kv_heads: int
+
+
+def _check_groups(seq_lens, group_starts, prefix_lens):
+    for name, t in (("seq_lens", seq_lens), ("group_starts", group_starts), ("prefix_lens", prefix_lens)):
+        if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.device != seq_lens.device:
+            raise ValueError(f"shared prefix: {name} must be an integer vector on {seq_lens.device}, got "
+                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    if group_starts.numel() != prefix_lens.numel() + 1:
+        raise ValueError(f"shared prefix: {prefix_lens.numel()} prefix lengths need {prefix_lens.numel() + 1} group "
+                         f"starts, got {group_starts.numel()}")
+
+
+def shared_prefix_plan(seq_lens, group_starts, prefix_lens, num_heads: int, num_kv_heads: int) -> SharedPrefixPlan:
+    """Plan the attention of one decode step: which CTA takes which keys of which rows.
+
+    The plan depends on the lengths alone (read on the device, without a synchronisation), so one
+    plan serves every layer of the step; lengths that change need a new one.  GPU only."""
+    _check_groups(seq_lens, group_starts, prefix_lens)
+    i32 = [t.to(torch.int32).contiguous() for t in (group_starts, prefix_lens, seq_lens)]
+    buf = ext().shared_prefix_plan(*i32, int(num_heads), int(num_kv_heads))
+    return SharedPrefixPlan(buf, seq_lens.numel(), prefix_lens.numel(), int(num_heads), int(num_kv_heads))
+
+
+def shared_prefix_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, group_starts, prefix_lens,
+                                   scale: Optional[float] = None, k_scale: float = 1.0, v_scale: float = 1.0,
+                                   plan: Optional[SharedPrefixPlan] = None):
+    """:func:`paged_decode_attention` for rows that share prefixes, each read once for its group.
+
+    ``q [B, nq, hd]`` (bf16 on a GPU), caches ``[blocks, block_size, nkv, hd]`` (bf16, or e4m3 with
+    ``k_scale`` / ``v_scale``), ``block_tables [B, max_blocks]`` (complete for every row, its prefix
+    included), ``seq_lens [B]``, ``group_starts [G+1]`` ascending, ``prefix_lens [G]``: the rows from
+    ``group_starts[g]`` up to ``group_starts[g+1]`` hold equal keys and values in their first
+    ``prefix_lens[g]`` positions, on the same pages or on copies.  Rows outside every group attend
+    alone; a row of length 0 gives zeros and bounds no group.  A prefix longer than a row of its
+    group is shared up to that row's length.
+
+    ``plan`` (:func:`shared_prefix_plan` of the same lengths) saves planning once per layer; it is
+    followed whatever the lengths are now.  Lengths and tables are device data: a table entry
+    outside the cache or group starts that descend are not followed but reported by
+    :func:`rl_b200.ops._ext.check_device_errors`.
+    """
+    _check_groups(seq_lens, group_starts, prefix_lens)
+    B = q.shape[0] if q.dim() == 3 else -1
+    if B < 0 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or q.shape[2] != k_cache.shape[3] \
+            or k_cache.shape[2] == 0 or q.shape[1] % k_cache.shape[2]:
+        raise ValueError(f"shared prefix attention: q {tuple(q.shape)} with caches {tuple(k_cache.shape)}, "
+                         f"{tuple(v_cache.shape)}")
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or seq_lens.numel() != B:
+        raise ValueError(f"shared prefix attention: {B} queries, block tables {tuple(block_tables.shape)}, "
+                         f"{seq_lens.numel()} lengths")
+    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    if not use_native(q):
+        if k_cache.dtype == torch.float8_e4m3fn:
+            k_cache, v_cache = k_cache.float() * k_scale, v_cache.float() * v_scale
+        out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+        live = seq_lens > 0
+        if bool(live.any()):  # every row's table is complete: the grouping changes what is read, not the result
+            out[live] = paged_decode_attention_ref(q[live], k_cache, v_cache, block_tables[live], seq_lens[live], scale)
+        return out
+    nq, nkv = q.shape[1], k_cache.shape[2]
+    if plan is None:
+        plan = shared_prefix_plan(seq_lens, group_starts, prefix_lens, nq, nkv)
+    elif plan[1:] != (B, prefix_lens.numel(), nq, nkv):
+        raise ValueError(f"shared prefix attention: a plan for (rows, groups, heads, KV heads) {plan[1:]} used for "
+                         f"{(B, prefix_lens.numel(), nq, nkv)}")
+    if q.stride(2) != 1 or q.stride(1) % 2 or q.stride(0) % 2 or q.data_ptr() % 4:
+        q = q.contiguous() if not q.is_contiguous() else q.clone()
+    return ext().shared_prefix_attn(q, k_cache, v_cache, block_tables.to(torch.int32).contiguous(), plan.buf,
+                                    plan.groups, float(scale), float(k_scale), float(v_scale))

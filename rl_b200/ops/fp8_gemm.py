@@ -29,7 +29,7 @@ from rl_b200.ops._ext import ext, use_native
 from rl_b200.ops.quant import quant_fp8_group, quant_fp8_group_ref
 
 __all__ = ["gemm_fp8", "gemm_fp8_ref", "fp8_linear", "gemm_mxf8", "quant_act_mx", "mx_weight_scales",
-           "fp8_linear_mx"]
+           "fp8_linear_mx", "fp8_linear_quantised"]
 
 
 def gemm_fp8_ref(a_q: torch.Tensor, a_s: torch.Tensor, b_q: torch.Tensor, b_s: torch.Tensor) -> torch.Tensor:
@@ -98,3 +98,12 @@ def fp8_linear_mx(x: torch.Tensor, w_q: torch.Tensor, w_s_t: torch.Tensor) -> to
     a_q, a_s_t = quant_act_mx(x.reshape(-1, shp[-1]))
     y = gemm_mxf8(a_q, a_s_t, w_q, w_s_t)
     return y.reshape(*shp[:-1], w_q.shape[0])
+
+
+def fp8_linear_quantised(q: torch.Tensor, scales: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor,
+                         mx: bool) -> torch.Tensor:
+    """:func:`fp8_linear_mx` (``mx``) or :func:`fp8_linear` of an input that is already e4m3
+    ``[.., K]`` with its scales (``rms_norm_fp8``)."""
+    q2 = q.reshape(-1, q.shape[-1])
+    y = gemm_mxf8(q2, scales, w_q, w_s) if mx else gemm_fp8(q2, scales, w_q, w_s)
+    return y.reshape(*q.shape[:-1], w_q.shape[0])

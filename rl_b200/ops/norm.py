@@ -5,6 +5,10 @@ component N7 of the survey; called through MCore layers built in
 ``nemo_rl/models/megatron/setup.py:2520``).  On CUDA tensors the forward and
 backward run in ``csrc/norm.cu``; the backward produces ``dx`` and a per-block
 fp32 partial of ``dw`` that is reduced in the same launch sequence.
+
+``rms_norm_fp8`` / ``add_rms_norm_fp8`` are the rollout's norms in front of an fp8
+projection: the normalised rows leave as e4m3 values with one scale per 128 of
+them, in one kernel and one pass over the residual stream.
 """
 
 from __future__ import annotations
@@ -13,7 +17,7 @@ import torch
 
 from rl_b200.ops._ext import ext, use_native
 
-__all__ = ["rms_norm", "add_rms_norm", "rms_norm_ref", "add_rms_norm_ref"]
+__all__ = ["rms_norm", "add_rms_norm", "rms_norm_ref", "add_rms_norm_ref", "rms_norm_fp8", "add_rms_norm_fp8"]
 
 
 def rms_norm_ref(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
@@ -89,3 +93,51 @@ def add_rms_norm(x: torch.Tensor, delta: torch.Tensor, w: torch.Tensor, eps: flo
     if use_native(x):
         return _AddRMSNorm.apply(x, delta, w, eps)
     return add_rms_norm_ref(x, delta, w, eps)
+
+
+def _norm_fp8(x: torch.Tensor, delta, w: torch.Tensor, eps: float, mx: bool):
+    H = x.shape[-1]
+    if x.dim() < 1 or H % 128 or H == 0:
+        raise ValueError(f"rms_norm_fp8: the hidden size must be a multiple of 128, got shape {tuple(x.shape)}")
+    if w.shape != (H,) or w.dtype != x.dtype or w.device != x.device:
+        raise ValueError(f"rms_norm_fp8: weight {tuple(w.shape)} {w.dtype} on {w.device} for input "
+                         f"{tuple(x.shape)} {x.dtype} on {x.device}")
+    if delta is not None and (delta.shape != x.shape or delta.dtype != x.dtype or delta.device != x.device):
+        raise ValueError(f"rms_norm_fp8: delta {tuple(delta.shape)} {delta.dtype} on {delta.device} for input "
+                         f"{tuple(x.shape)} {x.dtype} on {x.device}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, delta, w)):
+        raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad() (rollout only)")
+    if not use_native(x):
+        from rl_b200.ops.fp8_gemm import quant_act_mx
+        from rl_b200.ops.quant import quant_fp8_group_ref
+
+        y, s = (rms_norm_ref(x, w, eps), None) if delta is None else add_rms_norm_ref(x, delta, w, eps)
+        y2 = y.reshape(-1, H)
+        q, sc = quant_act_mx(y2) if mx else quant_fp8_group_ref(y2, 128, False)
+        return q.view(x.shape), sc, s
+
+    def rows(t):
+        t = t.reshape(-1, H).contiguous()
+        return t if t.data_ptr() % (8 * t.element_size()) == 0 else t.clone()
+
+    wc = w.contiguous()
+    wc = wc if wc.data_ptr() % (8 * wc.element_size()) == 0 else wc.clone()
+    out = ext().rmsnorm_fp8(rows(x), None if delta is None else rows(delta), wc, float(eps), bool(mx), bool(mx))
+    return out[0].view(x.shape), out[1], None if delta is None else out[2].view(x.shape)
+
+
+def rms_norm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, mx: bool = True):
+    """``rmsnorm(x) * w`` (rounded to ``x.dtype``) as e4m3 values with one scale per 128:
+    ``(q like x, scales)``.
+
+    ``mx``: power-of-two scales in the MN-major layout of :func:`rl_b200.ops.fp8_gemm.gemm_mxf8`
+    (``[H/128, rows rounded up to 128]``, padding 1); otherwise fp32 scales ``[rows, H/128]`` for
+    :func:`rl_b200.ops.fp8_gemm.gemm_fp8`.  The hidden size is a multiple of 128 (at most 16384 on a
+    GPU).  For inference: an input that needs a gradient is refused.
+    """
+    return _norm_fp8(x, None, w, eps, mx)[:2]
+
+
+def add_rms_norm_fp8(x: torch.Tensor, delta: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, mx: bool = True):
+    """``(q, scales, x + delta)``: :func:`rms_norm_fp8` of the residual sum, which is returned too."""
+    return _norm_fp8(x, delta, w, eps, mx)

@@ -1,0 +1,124 @@
+"""Group-rollout operators on the CPU: what they refuse, and their plain paths
+(shared-prefix decode attention, cache-page copies, RMSNorm with an fp8 output)."""
+
+import math
+
+import pytest
+import torch
+
+from rl_b200.ops.attention import paged_decode_attention_ref, shared_prefix_decode_attention
+from rl_b200.ops.cache_pages import copy_cache_pages
+from rl_b200.ops.norm import add_rms_norm_fp8, rms_norm_fp8
+
+
+def _attn_inputs(B=3, nq=4, nkv=2, hd=8, bs=4, width=3):
+    g = torch.Generator().manual_seed(0)
+    kc = torch.randn(B * width + 1, bs, nkv, hd, generator=g)
+    vc = torch.randn(B * width + 1, bs, nkv, hd, generator=g)
+    bt = torch.arange(B * width, dtype=torch.int32).view(B, width) + 1
+    return torch.randn(B, nq, hd, generator=g), kc, vc, bt
+
+
+def test_shared_prefix_attention_is_paged_attention_of_complete_tables():
+    q, kc, vc, bt = _attn_inputs()
+    lens = torch.tensor([12, 0, 5], dtype=torch.int32)
+    starts, prefix = torch.tensor([0, 3], dtype=torch.int32), torch.tensor([5], dtype=torch.int32)
+    out = shared_prefix_decode_attention(q, kc, vc, bt, lens, starts, prefix)
+    ref = paged_decode_attention_ref(q[[0, 2]], kc, vc, bt[[0, 2]], lens[[0, 2]])
+    assert torch.equal(out[[0, 2]], ref) and not out[1].any()
+    # fp8 caches are dequantised with their scales
+    k8, v8 = (kc / 0.02).clamp(-448, 448).to(torch.float8_e4m3fn), (vc / 0.02).clamp(-448, 448).to(torch.float8_e4m3fn)
+    o8 = shared_prefix_decode_attention(q, k8, v8, bt, lens, starts, prefix, k_scale=0.02, v_scale=0.02)
+    r8 = paged_decode_attention_ref(q[:1], k8.float() * 0.02, v8.float() * 0.02, bt[:1], lens[:1], 1 / math.sqrt(8))
+    assert torch.equal(o8[:1], r8)
+
+
+@pytest.mark.parametrize("change", ["starts_len", "starts_dtype", "lens_dim", "tables_rows", "heads", "head_dim",
+                                    "v_shape", "q_dim", "lens_count"])
+def test_shared_prefix_attention_refuses(change):
+    q, kc, vc, bt = _attn_inputs()
+    a = dict(q=q, k_cache=kc, v_cache=vc, block_tables=bt, seq_lens=torch.tensor([12, 3, 5], dtype=torch.int32),
+             group_starts=torch.tensor([0, 3], dtype=torch.int32), prefix_lens=torch.tensor([3], dtype=torch.int32))
+    shared_prefix_decode_attention(**a)
+    a.update({"starts_len": {"group_starts": torch.tensor([0, 2, 3], dtype=torch.int32)},
+              "starts_dtype": {"group_starts": torch.tensor([0.0, 3.0])},
+              "lens_dim": {"seq_lens": torch.tensor([[12, 3, 5]], dtype=torch.int32)},
+              "tables_rows": {"block_tables": bt[:2]},
+              "heads": {"q": q[:, :3]},
+              "head_dim": {"q": q[..., :4]},
+              "v_shape": {"v_cache": vc[:4]},
+              "q_dim": {"q": q[0]},
+              "lens_count": {"seq_lens": torch.tensor([12, 3], dtype=torch.int32)}}[change])
+    with pytest.raises(ValueError):
+        shared_prefix_decode_attention(**a)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float8_e4m3fn])
+def test_copy_cache_pages(dtype):
+    cache = torch.randn(3, 2, 7, 4, 2, 5).to(dtype)
+    want = cache.float()
+    want[:, :, 5] = want[:, :, 1]
+    want[:, :, 6, :2] = want[:, :, 1, :2]
+    want[:, :, 0, :1] = want[:, :, 2, :1]
+    copy_cache_pages(cache, [1, 1, 2, 3], torch.tensor([5, 6, 0, 4]), [4, 2, 1, 0])
+    assert torch.equal(cache.float(), want)
+    copy_cache_pages(cache, [], [])
+    assert torch.equal(cache.float(), want)
+    copy_cache_pages(cache, [6], [0])  # whole pages without token counts
+    want[:, :, 0] = want[:, :, 6]
+    assert torch.equal(cache.float(), want)
+
+
+@pytest.mark.parametrize("src,dst,tokens,error", [
+    ([1], [7], None, IndexError), ([-1], [2], None, IndexError), ([1], [2], [5], ValueError),
+    ([1], [2], [-1], ValueError), ([1, 3], [2, 2], None, ValueError), ([1, 2], [2, 3], None, ValueError),
+    ([1], [1], None, ValueError), ([1, 2], [3], None, ValueError), ([1], [3], [1, 1], ValueError),
+    (torch.tensor([1.0]), [2], None, ValueError), (torch.tensor([[1]]), [2], None, ValueError)])
+def test_copy_cache_pages_refuses(src, dst, tokens, error):
+    cache = torch.randn(2, 2, 7, 4, 2, 4)
+    before = cache.clone()
+    with pytest.raises(error):
+        copy_cache_pages(cache, src, dst, tokens)
+    assert torch.equal(cache, before)
+
+
+def test_copy_cache_pages_refuses_strided_caches():
+    with pytest.raises(ValueError):
+        copy_cache_pages(torch.zeros(2, 2, 7, 4, 2, 8)[..., :4], [1], [2])
+    with pytest.raises(ValueError):
+        copy_cache_pages(torch.zeros(7, 4, 2), [1], [2])
+
+
+@pytest.mark.parametrize("mx", [True, False])
+def test_norm_fp8_is_norm_then_quantisation(mx):
+    from rl_b200.ops.fp8_gemm import fp8_linear, fp8_linear_mx, fp8_linear_quantised, mx_weight_scales
+    from rl_b200.ops.norm import add_rms_norm, rms_norm
+    from rl_b200.ops.quant import quant_fp8_block
+
+    g = torch.Generator().manual_seed(0)
+    x, d = (torch.randn(2, 3, 256, generator=g, dtype=torch.float32).bfloat16() for _ in range(2))
+    w = torch.ones(256).bfloat16()
+    w_q, w_s = quant_fp8_block(torch.randn(40, 256, generator=g), 128, mx)
+    w_s = mx_weight_scales(w_s) if mx else w_s
+    linear = fp8_linear_mx if mx else fp8_linear
+    q, sc, s = add_rms_norm_fp8(x, d, w, mx=mx)
+    h, s_ref = add_rms_norm(x, d, w)
+    assert torch.equal(s, s_ref) and q.shape == x.shape and q.dtype == torch.float8_e4m3fn
+    assert torch.equal(fp8_linear_quantised(q, sc, w_q, w_s, mx), linear(h, w_q, w_s))
+    q, sc = rms_norm_fp8(x, w, mx=mx)
+    assert torch.equal(fp8_linear_quantised(q, sc, w_q, w_s, mx), linear(rms_norm(x, w), w_q, w_s))
+
+
+def test_norm_fp8_refuses():
+    x, w = torch.zeros(2, 256), torch.ones(256)
+    for args in ((torch.zeros(2, 200), torch.ones(200)), (x, torch.ones(128)), (x, w.double())):
+        with pytest.raises(ValueError):
+            rms_norm_fp8(*args)
+    with pytest.raises(ValueError):
+        add_rms_norm_fp8(x, torch.zeros(3, 256), w)
+    with pytest.raises(ValueError):
+        add_rms_norm_fp8(x, x.bfloat16(), w)
+    with pytest.raises(RuntimeError):
+        rms_norm_fp8(x.requires_grad_(True), w)
+    with torch.no_grad():
+        rms_norm_fp8(x, w)
