@@ -156,6 +156,13 @@ rmsnorm_fwd_rowcta_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat
 template <typename T>
 struct alignas(8 * sizeof(T)) Vec8 {
   T v[8];
+  // keeps the values packed: without it the compiler holds a second, unpacked copy of the row
+  // in registers from one phase to the next
+  __device__ __forceinline__ void keep() {
+    uint32_t* p = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+    for (int i = 0; i < (int)(8 * sizeof(T) / 4); ++i) asm volatile("" : "+r"(p[i]));
+  }
 };
 
 template <typename T, int NV, int TPR>
@@ -200,43 +207,62 @@ rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T
         const float v = to_f(f[k].v[i]);
         ss += v * v;
       }
+      f[k].keep();
     }
   }
   ss = TPR == 128 ? block_sum(ss, red) : warp_sum(ss);
   const float r = rsqrtf(ss / H + eps);
-  uint2* qr = reinterpret_cast<uint2*>(q + (size_t)row * H);
+  // y takes the row's place; its largest magnitudes, one per vector, then per 16 lanes.
+  // H % 128 == 0: a half-warp's 16 vectors are all inside the row or all outside.
+  float amax[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int j = t + k * TPR;
-    float y[8], amax = 0.f;
+    amax[k] = 0.f;
     if (j < nv) {
       const Vec8<T> g = wr[j];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        y[i] = to_f(from_f<T>(to_f(f[k].v[i]) * r * to_f(g.v[i])));
-        amax = fmaxf(amax, fabsf(y[i]));
+        f[k].v[i] = from_f<T>(to_f(f[k].v[i]) * r * to_f(g.v[i]));
+        amax[k] = fmaxf(amax[k], fabsf(to_f(f[k].v[i])));
       }
+      f[k].keep();
     }
-    // H % 128 == 0: a half-warp's 16 vectors are all inside the row or all outside
+  }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax[k] = fmaxf(amax[k], __shfl_xor_sync(0xffffffffu, amax[k], o));
+  // lane k of a half-warp does the two divisions of its k-th scale and hands the inverse round
+  const int lane16 = t & 15;
+  float inv[(NV + 15) / 16];
+#pragma unroll
+  for (int c = 0; c < (NV + 15) / 16; ++c) {
+    float m = 0.f;
+#pragma unroll
+    for (int k = 16 * c; k < NV && k < 16 * c + 16; ++k) m = lane16 == k - 16 * c ? amax[k] : m;
+    const float sc = fp8_scale(m, pow2);
+    inv[c] = 1.f / sc;
+    const int g = ((t & ~15) + (16 * c + lane16) * TPR) >> 4;
+    if (16 * c + lane16 < NV && g < ngroups) scales[ld ? (size_t)g * ld + row : (size_t)row * ngroups + g] = sc;
+  }
+  uint2* qr = reinterpret_cast<uint2*>(q + (size_t)row * H);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int j = t + k * TPR;
+    const float iv = __shfl_sync(0xffffffffu, inv[k / 16], k % 16, 16);
     if (j < nv) {
-      const float sc = fp8_scale(amax, pow2);
-      const float inv = 1.f / sc;
       uint32_t p[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h] * inv, y[4 * h + 1] * inv), __NV_SATFINITE,
+        const T* y = f[k].v + 4 * h;
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(to_f(y[0]) * iv, to_f(y[1]) * iv), __NV_SATFINITE,
                                                      __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h + 2] * inv, y[4 * h + 3] * inv),
-                                                     __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(to_f(y[2]) * iv, to_f(y[3]) * iv), __NV_SATFINITE,
+                                                     __NV_E4M3);
         p[h] = lo | (hi << 16);
       }
       qr[j] = make_uint2(p[0], p[1]);
-      if ((t & 15) == 0) {
-        const int g = j >> 4;
-        scales[ld ? (size_t)g * ld + row : (size_t)row * ngroups + g] = sc;
-      }
     }
   }
 }
@@ -385,25 +411,30 @@ std::vector<at::Tensor> add_rmsnorm_fwd(at::Tensor x, at::Tensor delta, at::Tens
   return {y, s, rstd};
 }
 
-// (q [rows, H] e4m3, scales fp32 [rows, H/128] or, mn_major, [H/128, rows rounded up to 128],
-//  s = x + delta when delta is given)
+// x [.., H] -> (q like x in e4m3, scales fp32 [rows, H/128] or, mn_major, [H/128, rows rounded up to
+// 128], s = x + delta when delta is given)
 std::vector<at::Tensor> rmsnorm_fp8(at::Tensor x, c10::optional<at::Tensor> delta, at::Tensor w, double eps, bool pow2,
                                     bool mn_major) {
-  check_rows(x, w);
-  RLB_CHECK(w.is_cuda() && w.device() == x.device() && w.is_contiguous(), "rmsnorm_fp8: weight on another device");
   const bool add = delta.has_value() && delta->defined();
+  const int64_t H = x.dim() > 0 ? x.size(-1) : 0;
+  RLB_CHECK(H >= 128 && H % 128 == 0 && H <= 16384, "rmsnorm_fp8: hidden size must be a multiple of 128, at most 16384");
+  RLB_CHECK(x.is_cuda() && w.dim() == 1 && w.size(0) == H && w.scalar_type() == x.scalar_type() && w.device() == x.device(),
+            "rmsnorm_fp8: weight mismatch");
   if (add)
-    RLB_CHECK(delta->sizes() == x.sizes() && delta->is_contiguous() && delta->scalar_type() == x.scalar_type() &&
-                  delta->device() == x.device(),
+    RLB_CHECK(delta->sizes() == x.sizes() && delta->scalar_type() == x.scalar_type() && delta->device() == x.device(),
               "rmsnorm_fp8: delta must match the input");
-  const int H = x.size(1);
-  RLB_CHECK(H % 128 == 0 && H >= 128 && H <= 16384, "rmsnorm_fp8: hidden size must be a multiple of 128, at most 16384");
-  RLB_CHECK(x.size(0) <= 0x7fffff00LL, "rmsnorm_fp8: too many rows");
-  const int64_t align = 8 * x.element_size();
-  for (const at::Tensor& t : {x, w, add ? *delta : x})
-    RLB_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % align == 0, "rmsnorm_fp8: tensors must be aligned to 8 values");
+  const int64_t n_rows = x.numel() / H;
+  RLB_CHECK(n_rows <= 0x7fffff00LL, "rmsnorm_fp8: too many rows");
   const c10::cuda::CUDAGuard g(x.device());
-  const int rows = x.size(0);
+  const uintptr_t align = 8 * x.element_size();
+  auto rows_of = [&](const at::Tensor& t) {  // contiguous, aligned to 8 values
+    at::Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % align ? c.clone() : c;
+  };
+  x = rows_of(x);
+  w = rows_of(w);
+  const at::Tensor d = add ? rows_of(*delta) : at::Tensor();
+  const int rows = (int)n_rows;
   const int ld = mn_major ? std::max(128, (rows + 127) / 128 * 128) : 0;
   auto f32 = x.options().dtype(at::kFloat);
   auto q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
@@ -420,9 +451,9 @@ std::vector<at::Tensor> rmsnorm_fp8(at::Tensor x, c10::optional<at::Tensor> delt
     auto launch = [&](auto nv, auto tpr) {
       constexpr int NV = decltype(nv)::value, TPR = decltype(tpr)::value;
       rmsnorm_fp8_kernel<scalar_t, NV, TPR><<<TPR == 128 ? out_rows : (out_rows + 3) / 4, 128, 0, stream()>>>(
-          (const scalar_t*)x.data_ptr(), add ? (const scalar_t*)delta->data_ptr() : nullptr,
+          (const scalar_t*)x.data_ptr(), add ? (const scalar_t*)d.data_ptr() : nullptr,
           (const scalar_t*)w.data_ptr(), add ? (scalar_t*)s.data_ptr() : nullptr, (__nv_fp8_e4m3*)q.data_ptr(),
-          scales.data_ptr<float>(), rows, H, (float)eps, pow2, ld);
+          scales.data_ptr<float>(), rows, (int)H, (float)eps, pow2, ld);
     };
     using std::integral_constant;
     if (cta) {

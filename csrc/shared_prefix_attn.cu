@@ -5,20 +5,22 @@
 // over row b's keys, of which the first P are the same for every row of its group.
 // The keys [0, P) of a group are read once for all of its rows: their queries form
 // the M side of a matrix product.  Keys [P, L_b) are read per row.  Both kinds of work
-// are units of 64-key tiles:
+// are units of 64- or 128-key tiles:
 //
-//   prefix unit: 64 query rows (row, head of one KV head) x the group's prefix
+//   prefix unit: MR query rows (row, head of one KV head) x the group's prefix
 //   suffix unit: the G query heads of one KV head of one row x the row's own keys
 //
-// spread over the CTAs by a plan: the tiles of all (unit, KV head) are laid on one
-// line and cut into equal runs, one per CTA, so ragged lengths balance and a long
-// prefix is split over many CTAs.  Each CTA leaves, per unit it touched, the fp32
-// partial (max, sum, unnormalised output) of an online softmax in base 2; the
-// combine kernel joins a row's partials in the order of its keys.  No atomics: the
-// result does not depend on timing.
+// spread over the CTAs by a plan: the tiles of all (prefix unit, KV head) are laid on one
+// line, those of all (suffix unit, KV head) on another, and each line is cut into equal
+// runs, one per CTA.  So every CTA has the same share of both kinds, ragged lengths
+// balance, and a long prefix is split over many CTAs.  Each CTA leaves, per unit it
+// touched, the fp32 partial (max, sum, unnormalised output) of an online softmax in
+// base 2; the combine kernel joins a row's partials in the order of its keys.  No
+// atomics: the result does not depend on timing.
 //
-// shared_prefix_plan_kernel   group bounds, unit list, tile offsets, every CTA's first unit
-// shared_prefix_attn_kernel   one producer warp (TMA) and four mma.sync warps
+// shared_prefix_plan_kernel     group bounds, unit list, tile offsets, every CTA's first units
+// shared_prefix_tc_kernel       64 or 128 dims, pages of a multiple of 8 keys: tcgen05
+// shared_prefix_attn_kernel     everything else: mma.sync
 // shared_prefix_combine_kernel  one warp per (row, head)
 //
 // The plan depends on the lengths only: one plan serves all layers of a decode step.
@@ -30,70 +32,87 @@ namespace sp {
 using namespace rlb::tc;
 typedef __nv_bfloat16 bf16;
 
-constexpr int BT = 64;        // keys per tile; a prefix is shared in whole tiles
+constexpr int BT = 64;        // a prefix is shared in multiples of these; keys per tile of the general kernel
 constexpr int MR = 64;        // query rows of a prefix unit
+constexpr int kMaxHeads = 64; // query heads per KV head
 constexpr int kUnitInts = 8;  // first tile, tiles, first key, keys' end, table row, first row, first query row, query rows
-constexpr int kRowInts = 4;   // group's first unit (-1: none), group's first row
-constexpr int kHeader = 8;    // tiles per CTA, tiles in all
+constexpr int kRowInts = 4;   // group's first unit (-1: none), group's first row, whether the row has keys
+constexpr int kHeader = 8;    // prefix: tiles per CTA, tiles in all; suffix: the same
 
 __device__ int g_shared_prefix_error = 0;
 constexpr int kErrGroups = 1, kErrPage = 2, kErrWait = 3;  // error words
 
+// What differs between the plans of the two kernels: CTAs, keys per tile.
+struct Shape {
+  int ctas, tile;
+};
+Shape shape_of(bool tc) { return tc ? Shape{num_sms(), 128} : Shape{2 * num_sms(), BT}; }
+bool use_tc(int64_t hd, int64_t block) { return (hd == 64 || hd == 128) && block % 8 == 0; }
+
+// where the units start in a plan
+__host__ __device__ inline int unit_offset(int ctas) { return kHeader + (2 * ctas + 3) / 4 * 4; }
 __host__ __device__ inline int max_chunks(int B, int G, int Gq) { return G + (B * Gq + MR - 1) / MR; }
 
 // ------------------------------------------------------------------------- plan
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 512;
 
 // inclusive scan of one value per thread (sum, or running maximum)
-template <bool MAX>
-__device__ __forceinline__ int block_scan(int v, int* s_warp) {
+template <bool MAX, typename T>
+__device__ __forceinline__ T block_scan(T v, T* s_warp) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    const T u = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v = MAX ? max(v, u) : v + u;
   }
   __syncthreads();
   if (lane == 31) s_warp[w] = v;
   __syncthreads();
-  if (w == 0) {
-    int x = s_warp[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x = MAX ? max(x, u) : x + u;
-    }
-    s_warp[lane] = x;
-  }
-  __syncthreads();
-  if (w > 0) v = MAX ? max(v, s_warp[w - 1]) : v + s_warp[w - 1];
-  return v;
+  T before = MAX ? v : (T)0;
+  for (int i = 0; i < w; ++i) before = MAX ? max(before, s_warp[i]) : before + s_warp[i];
+  return MAX ? before : before + v;
 }
 
-// plan: [kHeader][first unit of each CTA: ctas][units x kUnitInts][rows x kRowInts]
+// last entry of the ascending a[0..n) that is at most x
+__device__ __forceinline__ int last_at_most(const int* a, int n, int x) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] <= x) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo - 1;
+}
+
+// plan: [kHeader][first prefix unit of each CTA][first suffix unit of each CTA][units x kUnitInts][rows x kRowInts]
 __global__ void __launch_bounds__(kPlanThreads)
 shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __restrict__ prefix_lens,
-                          const int* __restrict__ seq_lens, int G, int B, int Gq, int nkv, int ctas,
+                          const int* __restrict__ seq_lens, int G, int B, int Gq, int nkv, int ctas, int tile,
                           int* __restrict__ plan) {
-  extern __shared__ int s_mem[];  // [G+1] group starts, [G] prefix tiles, [G] leader, [units] first tile
+  extern __shared__ int s_mem[];
   __shared__ int s_warp[32];
+  __shared__ long long s_warp2[32];
   pdl_launch_dependents();
-  int* s_start = s_mem;
-  int* s_tiles = s_start + G + 1;
-  int* s_leader = s_tiles + G;
-  int* s_first = s_leader + G;
+  int* s_len = s_mem;            // [B]
+  int* s_start = s_len + B;      // [G + 1]
+  int* s_share = s_start + G + 1;  // [G] prefix length, then shared keys
+  int* s_leader = s_share + G;   // [G] a row whose table is read
+  int* s_unit0 = s_leader + G;   // [G]
+  int* s_first = s_unit0 + G;    // [units]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int nc_max = max_chunks(B, G, Gq), units = nc_max + B;
   int* cta_unit = plan + kHeader;
-  int* unit = cta_unit + ctas;
+  int* unit = plan + unit_offset(ctas);
   int* rowinfo = unit + units * kUnitInts;
+  for (int b = tid; b < B; b += kPlanThreads) s_len[b] = max(seq_lens[b], 0);
+  for (int g = tid; g < G; g += kPlanThreads) s_share[g] = max(prefix_lens[g], 0);
   // group starts, made ascending and kept inside [0, B]: groups never overlap
   int carry = 0;
   bool bad = false;
   for (int g0 = 0; g0 <= G; g0 += kPlanThreads) {
     const int g = g0 + tid;
     const int raw = g <= G ? group_starts[g] : 0;
-    int v = block_scan<true>(max(carry, min(max(raw, 0), B)), s_warp);
+    const int v = block_scan<true>(max(carry, min(max(raw, 0), B)), s_warp);
     if (g <= G) {
       s_start[g] = v;
       bad |= v != raw;
@@ -102,148 +121,124 @@ shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __res
     carry = s_start[min(G, g0 + kPlanThreads - 1)];
   }
   if (bad) atomicExch(&g_shared_prefix_error, kErrGroups);
-  for (int b = tid; b < B; b += kPlanThreads) {
-    rowinfo[b * kRowInts] = -1;
-    rowinfo[b * kRowInts + 1] = 0;
-  }
-  __syncthreads();
-  // a group shares the whole tiles that every live row of it has; one live row shares nothing
+  // a group shares what every live row of it has, in multiples of BT; one live row shares nothing
   for (int g = warp; g < G; g += kPlanThreads / 32) {
-    int len = max(prefix_lens[g], 0), live = 0, leader = B;
+    int len = s_share[g], live = 0, leader = B;
     for (int b = s_start[g] + lane; b < s_start[g + 1]; b += 32) {
-      const int L = seq_lens[b];
+      const int L = s_len[b];
       if (L > 0) {
         len = min(len, L);
         leader = min(leader, b);
         ++live;
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      len = min(len, __shfl_xor_sync(0xffffffffu, len, o));
-      leader = min(leader, __shfl_xor_sync(0xffffffffu, leader, o));
-      live += __shfl_xor_sync(0xffffffffu, live, o);
-    }
+    len = __reduce_min_sync(0xffffffffu, len);
+    leader = __reduce_min_sync(0xffffffffu, leader);
+    live = __reduce_add_sync(0xffffffffu, live);
     if (lane == 0) {
-      s_tiles[g] = live > 1 ? len / BT : 0;
+      s_share[g] = live > 1 ? len / BT * BT : 0;
       s_leader[g] = leader;
     }
   }
   __syncthreads();
   // prefix units: per group, ceil(rows * Gq / MR) chunks of its query rows
-  int unit_carry = 0, tile_carry = 0;
+  int unit_carry = 0, prefix_tiles = 0;
   for (int g0 = 0; g0 < G; g0 += kPlanThreads) {
     const int g = g0 + tid;
     int chunks = 0, n = 0, start = 0, rows = 0;
     if (g < G) {
       start = s_start[g];
       rows = (s_start[g + 1] - start) * Gq;
-      n = s_tiles[g];
+      n = (s_share[g] + tile - 1) / tile;
       chunks = n > 0 ? (rows + MR - 1) / MR : 0;
     }
-    const int uend = block_scan<false>(chunks, s_warp);
-    const int tend = block_scan<false>(chunks * n, s_warp);
-    const int u0 = unit_carry + uend - chunks, a0 = tile_carry + tend - chunks * n;
+    // both sums in one scan: units in the high half, tiles in the low one
+    const long long end = block_scan<false>(((long long)chunks << 32) + chunks * n, s_warp2);
+    const int u0 = unit_carry + (int)(end >> 32) - chunks, a0 = prefix_tiles + (int)end - chunks * n;
+    if (g < G) s_unit0[g] = u0;
     for (int c = 0; c < chunks; ++c) {
-      int* m = unit + (u0 + c) * kUnitInts;
-      s_first[u0 + c] = m[0] = a0 + c * n;
-      m[1] = n;
-      m[2] = 0;
-      m[3] = n * BT;
-      m[4] = s_leader[g];
-      m[5] = start;
-      m[6] = c * MR;
-      m[7] = min(MR, rows - c * MR);
-    }
-    if (chunks > 0)
-      for (int b = start; b < s_start[g + 1]; ++b) {
-        rowinfo[b * kRowInts] = u0;
-        rowinfo[b * kRowInts + 1] = start;
-      }
-    __syncthreads();
-    if (tid == kPlanThreads - 1) {
-      s_warp[0] = unit_carry + uend;
-      s_warp[1] = tile_carry + tend;
+      int4* m = reinterpret_cast<int4*>(unit + (u0 + c) * kUnitInts);
+      s_first[u0 + c] = a0 + c * n;
+      m[0] = make_int4(a0 + c * n, n, 0, s_share[g]);
+      m[1] = make_int4(s_leader[g], start, c * MR, min(MR, rows - c * MR));
     }
     __syncthreads();
-    unit_carry = s_warp[0];
-    tile_carry = s_warp[1];
+    if (tid == kPlanThreads - 1) s_warp2[0] = end;
+    __syncthreads();
+    unit_carry += (int)(s_warp2[0] >> 32);
+    prefix_tiles += (int)s_warp2[0];
     __syncthreads();
   }
   for (int u = unit_carry + tid; u < nc_max; u += kPlanThreads) {  // unused prefix units
-    int* m = unit + u * kUnitInts;
-    s_first[u] = m[0] = tile_carry;
-    m[1] = 0;
+    s_first[u] = prefix_tiles;
+    *reinterpret_cast<int4*>(unit + u * kUnitInts) = make_int4(prefix_tiles, 0, 0, 0);
   }
-  // suffix units: row b's keys behind its group's shared tiles
+  // suffix units: row b's keys behind its group's shared ones
+  int suffix_tiles = 0;
   for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
     const int b = b0 + tid;
-    int k0 = 0, k1 = 0;
+    int k0 = 0, k1 = 0, u0 = -1, start = 0;
     if (b < B) {
-      k1 = max(seq_lens[b], 0);
-      // the group of row b: the last one that starts at or before it
-      int lo = 0, hi = G;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s_start[mid] <= b) lo = mid + 1;
-        else hi = mid;
+      k1 = s_len[b];
+      const int g = last_at_most(s_start, G, b);
+      if (g >= 0 && b < s_start[g + 1] && s_share[g] > 0) {
+        k0 = min(s_share[g], k1);
+        u0 = s_unit0[g];
+        start = s_start[g];
       }
-      if (lo > 0 && b < s_start[lo]) k0 = min(s_tiles[lo - 1] * BT, k1);
     }
-    const int n = (k1 - k0 + BT - 1) / BT;
-    const int tend = block_scan<false>(n, s_warp);
+    const int n = (k1 - k0 + tile - 1) / tile;
+    const int end = block_scan<false>(n, s_warp);
     if (b < B) {
-      int* m = unit + (nc_max + b) * kUnitInts;
-      s_first[nc_max + b] = m[0] = tile_carry + tend - n;
-      m[1] = n;
-      m[2] = k0;
-      m[3] = k1;
-      m[4] = b;
-      m[5] = b;
-      m[6] = 0;
-      m[7] = Gq;
-      rowinfo[b * kRowInts + 2] = k1 > 0;
+      int4* m = reinterpret_cast<int4*>(unit + (nc_max + b) * kUnitInts);
+      const int a0 = suffix_tiles + end - n;
+      s_first[nc_max + b] = a0;
+      m[0] = make_int4(a0, n, k0, k1);
+      m[1] = make_int4(b, b, 0, Gq);
+      *reinterpret_cast<int4*>(rowinfo + b * kRowInts) = make_int4(u0, start, k1 > 0, 0);
     }
     __syncthreads();
-    if (tid == kPlanThreads - 1) s_warp[0] = tile_carry + tend;
+    if (tid == kPlanThreads - 1) s_warp[0] = end;
     __syncthreads();
-    tile_carry = s_warp[0];
+    suffix_tiles += s_warp[0];
     __syncthreads();
   }
-  const long long total = (long long)tile_carry * nkv;
-  const int per = (int)((total + ctas - 1) / ctas);
-  if (tid == 0) {
-    plan[0] = max(per, 1);
-    plan[1] = (int)total;
-  }
-  // every CTA's first unit: the last one that starts at or before its first tile
-  for (int i = tid; i < ctas; i += kPlanThreads) {
-    const long long x = (long long)i * max(per, 1);
+  const long long total0 = (long long)prefix_tiles * nkv, total1 = (long long)suffix_tiles * nkv;
+  const int per0 = max((int)((total0 + ctas - 1) / ctas), 1), per1 = max((int)((total1 + ctas - 1) / ctas), 1);
+  if (tid == 0) *reinterpret_cast<int4*>(plan) = make_int4(per0, (int)total0, per1, (int)total1);
+  // every CTA's first unit of each line: the last one that starts at or before its first tile
+  // (units without tiles start where the next one does, so this one has tiles)
+  for (int i = tid; i < 2 * ctas; i += kPlanThreads) {
+    const bool suffix = i >= ctas;
+    const long long x = (long long)(suffix ? i - ctas : i) * (suffix ? per1 : per0);
     int u = 0;
-    if (x < total) {
-      const int a = (int)(x / nkv);
-      int lo = 0, hi = units;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s_first[mid] <= a) lo = mid + 1;
-        else hi = mid;
-      }
-      u = lo - 1;
-    }
+    if (x < (suffix ? total1 : total0))
+      u = suffix ? nc_max + last_at_most(s_first + nc_max, B, (int)(x / nkv)) : last_at_most(s_first, nc_max, (int)(x / nkv));
     cta_unit[i] = u;
   }
 }
 
 // --------------------------------------------------------------------- attention
-__device__ __forceinline__ void tma_3d(uint32_t dst, const void* tmap, uint32_t mbar, int x, int y, int z) {
+// One lane of a converged warp.  The compiler knows this form: what the lane issues takes its operands
+// from uniform registers, where a plain "lane == 0" costs a move of each through a per-lane loop (measured: 50
+// to 75 cycles a matrix product of 16 to 64 columns, against 103).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t x;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(x));
+  return x != 0;
+}
+__device__ __forceinline__ void tma_4d(uint32_t dst, const void* tmap, uint32_t mbar, int head, int key, int span) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n" ::"r"(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n" ::"r"(
           dst),
-      "l"(tmap), "r"(mbar), "r"(x), "r"(y), "r"(z)
+      "l"(tmap), "r"(mbar), "r"(0), "r"(head), "r"(key), "r"(span)
       : "memory");
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_arrive(uint32_t mbar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(mbar) : "memory");
@@ -293,82 +288,199 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;\n" ::: "memory"); }
 
-template <int HD, bool F8>
-struct Cfg {
+// a stage of KT keys in shared memory
+template <int HD, bool F8, int KT>
+struct Tile {
+  static constexpr int KEYS = KT;
   static constexpr int RB = HD * (F8 ? 1 : 2);              // bytes of a key
   static constexpr int BOXB = RB < 128 ? RB : 128;          // bytes of a key in one box = its swizzle span
   static constexpr int NBOX = RB / BOXB;
+  static_assert(NBOX <= 2, "at most 256 bytes a key");
   static constexpr int CH = BOXB / 16;                      // 16-byte chunks of a box row
-  static constexpr int TILE = BT * RB;                      // bytes of K (or V) of a tile
-  // stages: as many as leave room for two CTAs on an SM, at most 8
-  static constexpr int RED = 2 * (HD / 4 + 2) * 32 * 4;     // merge buffer: two warps, half of the rows
-  static constexpr int FIT = (112 * 1024 - RED - 1024 - 256) / (2 * TILE);
-  static constexpr int ST = FIT < 8 ? FIT : 8;
-  static constexpr int SMEM = 1024 + ST * 2 * TILE + RED + 256;
-  static_assert(ST >= 2, "two stages at least");
+  static constexpr int BYTES = KT * RB;                     // of K (or V)
   // offset of chunk c of a key, as the TMA unit's swizzle (span BOXB) places it
   static __device__ __forceinline__ int at(int row, int c) {
     const int box = c / CH, cc = c % CH;
     const int x = CH == 8 ? (row & 7) : CH == 4 ? ((row >> 1) & 3) : ((row >> 2) & 1);
-    return box * BT * BOXB + (row * CH + (cc ^ x)) * 16;
+    return box * KT * BOXB + (row * CH + (cc ^ x)) * 16;
   }
 };
+
+template <int HD>
+constexpr int kRedBytes = 2 * (HD / 4 + 2) * 32 * 4;  // merge buffer: two warps, half of their rows
 
 struct Args {
   const bf16* q;
   long long q_row, q_head;  // strides
   const uint8_t *k, *v;     // caches (the path without TMA)
   const int* tables;
-  int table_row, n_blocks, block, box;  // table width, pages, keys per page, keys per TMA box (0: no TMA)
+  int table_row, n_blocks, block, box;  // table width, pages, keys per page, keys per TMA box of a tile (0: no TMA)
   const int* plan;
   int ctas, units, B, nq, nkv, Gq;
+  uint32_t inv_gq;  // ceil(2^32 / Gq): rr / Gq is the high word of rr * inv_gq for every query row rr of a group
   float scale_log2;
   float *part_o, *part_ml;
 };
 
-// a position on the line of tiles
+// a CTA's run on one of the two lines of tiles, and the position in it
 struct Cursor {
-  int u, kvh, j;                    // unit, KV head, tile
+  const int* unit;
+  int u, u_end, kvh, j;               // unit, KV head, tile
   int n, k0, k1, trow, row0, r0, rn;  // of the unit
-  __device__ __forceinline__ void load(const int* unit) {
+  int x, x1, nkv;                     // position, end of the run
+  __device__ __forceinline__ void load() {
     const int4 a = *reinterpret_cast<const int4*>(unit + u * kUnitInts);
     const int4 b = *reinterpret_cast<const int4*>(unit + u * kUnitInts + 4);
     n = a.y, k0 = a.z, k1 = a.w, trow = b.x, row0 = b.y, r0 = b.z, rn = b.w;
   }
-  __device__ __forceinline__ void seek(const int* unit, int first_unit, int x, int nkv) {
-    u = first_unit;
-    load(unit);
+  // line 0: prefix units, line 1: suffix units; false when the CTA has no tile of it
+  __device__ __forceinline__ bool begin(const Args& a, int line) {
+    const int per = a.plan[2 * line], total = a.plan[2 * line + 1];
+    nkv = a.nkv;
+    x = (int)min((long long)total, (long long)blockIdx.x * per);
+    x1 = min(total, x + per);
+    if (x >= x1) return false;
+    unit = a.plan + unit_offset(a.ctas);
+    u_end = line ? a.units : a.units - a.B;
+    u = a.plan[kHeader + line * a.ctas + blockIdx.x];
+    load();
     const int y = x - unit[u * kUnitInts] * nkv;
     kvh = y / n;
     j = y - kvh * n;
+    return true;
   }
-  // the next tile; false when it belongs to another segment (unit or KV head)
-  __device__ __forceinline__ bool next(const int* unit, int units, int nkv) {
-    if (++j < n) return true;
+  // to the next tile; true when it belongs to the same segment (unit, KV head and run)
+  __device__ __forceinline__ bool next() {
+    const bool more = ++x < x1;
+    if (++j < n) return more;
     j = 0;
-    if (++kvh < nkv) return false;
+    if (++kvh < nkv || !more) return false;
     kvh = 0;
     do {
-      if (++u >= units) return false;
-      load(unit);
+      if (++u >= u_end) return false;
+      load();
     } while (n == 0);
     return false;
   }
+  __device__ __forceinline__ bool done() const { return x >= x1; }
 };
 
-template <int HD, bool F8>
-struct Warp {  // a consumer warp's state: 16 query rows, HD dims
-  using C = Cfg<HD, F8>;
+// Where the partial of local query row rl of a segment goes: a slot of the row when the segment is its
+// unit's first, else a slot of the CTA.  sub: the tc kernel keeps two partials of a segment, of its
+// even and of its odd tiles.
+__device__ __forceinline__ long long partial_slot(const Args& a, const Cursor& s, int line, int sub, int rl) {
+  const int nqt = a.B * a.nq, ls = 2 * line + sub;
+  if (s.j > 0) return 4LL * nqt + ((long long)ls * a.ctas + blockIdx.x) * MR + rl;
+  const int r = s.r0 + rl;
+  return (long long)ls * nqt + (long long)(s.row0 + r / a.Gq) * a.nq + s.kvh * a.Gq + r % a.Gq;
+}
+
+// the pages of a unit, 32 table entries at a time, one per lane of the producer warp
+struct Pages {
+  int page0 = 0, ids = 0;
+  bool fresh = true;
+  // all lanes: the page of table entry p of row trow
+  __device__ __forceinline__ int get(const Args& a, int trow, int p) {
+    const int lane = threadIdx.x & 31;
+    if (fresh || p < page0 || p >= page0 + 32) {
+      page0 = p;
+      fresh = false;
+      ids = a.tables[(long long)trow * a.table_row + min(p + lane, a.table_row - 1)];
+    }
+    int b = __shfl_sync(0xffffffffu, ids, p - page0);
+    if (b < 0 || b >= a.n_blocks || p >= a.table_row) {  // reported; a page of the cache is read instead
+      if (lane == 0) atomicExch(&g_shared_prefix_error, kErrPage);
+      b = 0;
+    }
+    return b;
+  }
+};
+
+// The producer warp's walk over a line: the cursor, and the place of its next key in the cache.
+// Divisions by the page size happen once a segment; boxes of `box` keys divide pages and stages.
+struct Feed {
+  Cursor s;
+  Pages pages;
+  int key, off, p, z;  // next key, its offset in its page, that page's table entry, its place in the cache
+  int line;
+  bool valid;
+  __device__ __forceinline__ void seek(const Args& a, int tile) {
+    key = s.k0 + s.j * tile;
+    p = key / a.block;
+    off = key - p * a.block;
+    pages.fresh = true;
+    z = pages.get(a, s.trow, p) * a.block + off;
+  }
+  // the prefix line's run, then the suffix line's
+  __device__ __forceinline__ void begin(const Args& a, int tile, int from = 0) {
+    valid = false;
+    for (line = from; line < 2 && !valid; ++line) valid = s.begin(a, line);
+    --line;
+    if (valid) seek(a, tile);
+  }
+  // behind a tile's last key: to the next tile
+  __device__ __forceinline__ void next(const Args& a, int tile) {
+    if (s.next()) return;
+    if (!s.done()) seek(a, tile);
+    else begin(a, tile, line + 1);
+  }
+  // bytes of a load of up to C::KEYS keys
+  template <typename C>
+  __device__ __forceinline__ uint32_t bytes(int box) const {
+    return (uint32_t)((min(C::KEYS, s.k1 - key) + box - 1) / box * box * C::RB);
+  }
+  // the next KEYS keys (whole boxes, none behind the last key) of one cache
+  template <typename C>
+  __device__ __forceinline__ void load(const Args& a, const CUtensorMap* tm, int box, uint32_t dst, uint32_t bar) {
+    for (int r = 0; r < C::KEYS && key < s.k1; r += box) {
+      if (elect_one()) {  // a box that is the whole stage brings all spans of its keys, a smaller one goes span by span
+        tma_4d(dst + r * C::BOXB, tm, bar, s.kvh, z, 0);
+        if (C::NBOX > 1 && box < C::KEYS) tma_4d(dst + C::KEYS * C::BOXB + r * C::BOXB, tm, bar, s.kvh, z, 1);
+      }
+      __syncwarp();
+      key += box;
+      if (key < s.k1) {
+        off += box;
+        z += box;
+        if (off == a.block) {
+          off = 0;
+          z = pages.get(a, s.trow, ++p) * a.block;
+        }
+      }
+    }
+  }
+};
+
+// waits, within a limit, for the copies of stages [k - stages, k) that are still in flight (after an abort)
+__device__ __forceinline__ void drain(uint32_t bar_full, int stages, int k) {
+  for (int i = max(0, k - stages); i < k; ++i) {
+    const long long t0 = clock64();
+    while (!mbar_test(bar_full + 8 * (i % stages), (i / stages) & 1) && clock64() - t0 < kWaitCycles) {
+    }
+  }
+}
+
+// factor 2^(13 - exponent) that brings a row of q of largest magnitude mx near 2^13, where f16 keeps
+// 8-bit mantissas exact over 37 binades; infinities and NaN stay, tiny rows are scaled by 2^110
+__device__ __forceinline__ int f16_row_exponent(float mx) {
+  const int ex = (int)(__float_as_uint(mx) >> 23);
+  return ex == 255 ? 140 : max(ex, 30);
+}
+__device__ __forceinline__ float f16_row_factor(int ex) { return __uint_as_float((uint32_t)(267 - ex) << 23); }
+__device__ __forceinline__ float f16_row_inverse(int ex) { return __uint_as_float((uint32_t)(ex - 13) << 23); }
+
+template <int HD, bool F8, int KT>
+struct Warp {  // a consumer warp's state: 16 query rows, HD dims, stages of KT keys
+  using C = Tile<HD, F8, KT>;
   uint32_t q[HD / 16][4];
   float o[HD / 8][4];
   float m[2], l[2], c[2];  // running maximum (log2), partial sum, score factor of rows g and g + 8
   int lane, g, t;
 
   __device__ __forceinline__ void start(const Args& a, const Cursor& s, int wm) {
-    // Q fragments.  For an e4m3 cache the products run in f16 (an e4m3 value is exact there):
-    // each query row is scaled by a power of two to a maximum near 2^13, which keeps 8-bit
-    // mantissas exact over 37 binades, and its dims are taken in the order in which a lane holds
-    // four neighbouring bytes of a key.
+    // Q fragments.  For an e4m3 cache the products run in f16 (an e4m3 value is exact there): each
+    // query row is scaled by a power of two, and its dims are taken in the order in which a lane
+    // holds four neighbouring bytes of a key.
     const bf16* p[2];
     bool ok[2];
 #pragma unroll
@@ -403,10 +515,9 @@ struct Warp {  // a consumer warp's state: 16 query rows, HD dims
       for (int h = 0; h < 2; ++h) {
         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-        int ex = (int)(__float_as_uint(mx[h]) >> 23);  // biased exponent
-        ex = ex == 255 ? 140 : max(ex, 30);            // infinities stay; tiny rows are scaled by 2^110
-        f[h] = __uint_as_float((uint32_t)(127 + 140 - ex) << 23);   // 2^(13 - (ex - 127))
-        c[h] = a.scale_log2 * __uint_as_float((uint32_t)(127 - 140 + ex) << 23);
+        const int ex = f16_row_exponent(mx[h]);
+        f[h] = f16_row_factor(ex);
+        c[h] = a.scale_log2 * f16_row_inverse(ex);
       }
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk)
@@ -420,10 +531,10 @@ struct Warp {  // a consumer warp's state: 16 query rows, HD dims
     for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
   }
 
-  // keys [key0, key0 + BT / WK) of a tile of which the first nvalid are the row's
-  template <int WK, bool PART>
+  // keys [key0, key0 + NK) of a stage of which the first nvalid are the row's
+  template <int NK, bool PART>
   __device__ __forceinline__ void tile(uint32_t sk, uint32_t sv, int key0, int nvalid) {
-    constexpr int NT = BT / WK / 8;
+    constexpr int NT = NK / 8;
     float s[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
@@ -584,22 +695,49 @@ struct Warp {  // a consumer warp's state: 16 query rows, HD dims
   }
 };
 
+// joins the partials of the warps kq = 0 .. wk-1 that split the keys of the same rows into warp 0's;
+// all four warps call it
+template <typename W>
+__device__ __forceinline__ void join_warps(W& w, float* red, int stride, int wk, int wm, int kq, int rows) {
+  w.finish_sums();
+  for (int step = wk / 2; step > 0; step /= 2)
+    for (int h = 0; h < 2; ++h) {
+      if (h == 1 && rows <= 8) break;
+      float* buf = red + (wk == 4 ? kq % step : wm) * stride;
+      if (kq >= step && kq < 2 * step) w.put(buf, h);
+      consumers_sync();
+      if (kq < step) w.join(buf, h);
+      consumers_sync();
+    }
+}
+
+template <int HD, bool F8>
+struct Gen {  // shared memory of the general kernel: two CTAs on an SM
+  using C = Tile<HD, F8, BT>;
+  static constexpr int FIT = (112 * 1024 - kRedBytes<HD> - 1024 - 256) / (2 * C::BYTES);
+  static constexpr int ST = FIT < 8 ? FIT : 8;
+  static constexpr int SMEM = 1024 + ST * 2 * C::BYTES + kRedBytes<HD> + 256;
+  static_assert(ST >= 2, "two stages at least");
+};
+
+// One producer warp and four mma.sync warps, for every head size, page size and head count.
 template <int HD, bool F8>
 __global__ void __launch_bounds__(160, 2)
 shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                           const __grid_constant__ Args a) {
-  using C = Cfg<HD, F8>;
+  using C = Tile<HD, F8, BT>;
+  constexpr int ST = Gen<HD, F8>::ST;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
-  float* red = reinterpret_cast<float*>(smem_raw + (base - raw) + C::ST * 2 * C::TILE);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(red) + C::RED);
-  const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * C::ST;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * C::ST);
+  float* red = reinterpret_cast<float*>(smem_raw + (base - raw) + ST * 2 * C::BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(red) + kRedBytes<HD>);
+  const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * ST;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * ST);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::ST; ++s) {
+    for (int s = 0; s < ST; ++s) {
       mbar_init(bar_full + 8 * s, a.box ? 1 : 32);
       mbar_init(bar_empty + 8 * s, 4);
     }
@@ -608,57 +746,26 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
   }
   __syncthreads();
   pdl_wait();
-  const int per = a.plan[0], total = a.plan[1];
-  const int x0 = (int)min((long long)total, (long long)blockIdx.x * per), x1 = min(total, x0 + per);
-  if (x0 >= x1) return;
-  const int* unit = a.plan + kHeader + a.ctas;
-  Cursor s;
-  s.seek(unit, a.plan[kHeader + blockIdx.x], x0, a.nkv);
 
   if (warp == 4) {
-    // producer: the pages of a unit come 32 table entries at a time, one per lane
-    int page0 = -1, pages = 0;
-    bool fresh = true;
     int k = 0;
-    for (int x = x0; x < x1 && !*abort_flag; ++x, ++k) {
-      const int st = k % C::ST;
-      const int key = s.k0 + s.j * BT;
-      const int last = (min(key + BT, s.k1) - 1) / a.block;  // last page with keys of the tile
-      if (!mbar_wait_err(bar_empty + 8 * st, ((k / C::ST) & 1) ^ 1, abort_flag, &g_shared_prefix_error, kErrWait)) break;
-      const uint32_t sk = base + st * 2 * C::TILE, sv = sk + C::TILE;
-      auto page = [&](int p) {  // all lanes: the page of table entry p
-        if (fresh || p < page0 || p >= page0 + 32) {
-          page0 = p;
-          fresh = false;
-          const int e = min(p + lane, a.table_row - 1);
-          pages = a.tables[(long long)s.trow * a.table_row + e];
-        }
-        int b = __shfl_sync(0xffffffffu, pages, p - page0);
-        if (b < 0 || b >= a.n_blocks || p >= a.table_row) {  // reported; a page of the cache is read instead
-          if (lane == 0) atomicExch(&g_shared_prefix_error, kErrPage);
-          b = 0;
-        }
-        return b;
-      };
+    Feed f;
+    for (f.begin(a, BT); f.valid && !*abort_flag; ++k) {
+      const int st = k % ST;
+      if (!mbar_wait_err(bar_empty + 8 * st, ((k / ST) & 1) ^ 1, abort_flag, &g_shared_prefix_error, kErrWait)) break;
+      const uint32_t sk = base + st * 2 * C::BYTES, sv = sk + C::BYTES;
       if (a.box) {
-        if (lane == 0) mbar_expect_tx(bar_full + 8 * st, 2 * C::TILE);
-        for (int r = 0; r < BT; r += a.box) {
-          // boxes behind the last key re-read its page: they are masked
-          const int p = min((key + r) / a.block, last);
-          const int z = page(p) * a.block + (key + r) % a.block;
-          if (lane == 0)
-#pragma unroll
-            for (int b = 0; b < C::NBOX; ++b) {
-              const uint32_t off = b * BT * C::BOXB + r * C::BOXB;
-              tma_3d(sk + off, &tk, bar_full + 8 * st, b * (HD / C::NBOX), s.kvh, z);
-              tma_3d(sv + off, &tv, bar_full + 8 * st, b * (HD / C::NBOX), s.kvh, z);
-            }
-        }
+        if (elect_one()) mbar_expect_tx(bar_full + 8 * st, 2 * f.template bytes<C>(a.box));
+        __syncwarp();
+        Feed v = f;
+        v.template load<C>(a, &tv, a.box, sv, bar_full + 8 * st);
+        f.template load<C>(a, &tk, a.box, sk, bar_full + 8 * st);
       } else {
+        const int key = f.s.k0 + f.s.j * BT;
         for (int r = 0; r < BT; ++r) {
-          const int kr = min(key + r, s.k1 - 1);
-          const long long slot = (long long)page(kr / a.block) * a.block + kr % a.block;
-          const long long off = (slot * a.nkv + s.kvh) * C::RB;
+          const int kr = min(key + r, f.s.k1 - 1);
+          const long long slot = (long long)f.pages.get(a, f.s.trow, kr / a.block) * a.block + kr % a.block;
+          const long long off = (slot * a.nkv + f.s.kvh) * C::RB;
           for (int c = lane; c < 2 * (C::RB / 16); c += 32) {
             const int cc = c % (C::RB / 16);
             const bool is_v = c >= C::RB / 16;
@@ -667,87 +774,763 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
         }
         cp_async_arrive(bar_full + 8 * st);
       }
-      if (!s.next(unit, a.units, a.nkv)) fresh = true;
+      f.next(a, BT);
     }
-    if (*abort_flag)  // let the copies in flight land before the block leaves
-      for (int i = max(0, k - C::ST); i < k; ++i) {
-        const long long t0 = clock64();
-        while (!mbar_test(bar_full + 8 * (i % C::ST), (i / C::ST) & 1) && clock64() - t0 < kWaitCycles) {
-        }
-      }
+    if (*abort_flag) drain(bar_full, ST, k);
     return;
   }
 
-  Warp<HD, F8> w;
+  Warp<HD, F8, BT> w;
   w.lane = lane;
   w.g = lane >> 2;
   w.t = lane & 3;
-  const int nqt = a.B * a.nq;
-  bool first = true;
-  int wk = 1, wm = 0, kq = 0, j0 = 0;
-  for (int x = x0, k = 0; x < x1; ++x, ++k) {
-    const int st = k % C::ST;
-    if (first) {
+  int k = 0;
+  for (int line = 0; line < 2; ++line) {
+    Cursor s;
+    if (!s.begin(a, line)) continue;
+    while (!s.done()) {
       // 16 query rows a warp; with fewer rows than 64 the warps split the keys instead
-      wk = s.rn <= 16 ? 4 : s.rn <= 32 ? 2 : 1;
-      wm = warp / wk;
-      kq = warp % wk;
-      j0 = s.j;
-      w.start(a, s, wm);
-      first = false;
-    }
-    const uint32_t sk = base + st * 2 * C::TILE, sv = sk + C::TILE;
-    const int nvalid = s.k1 - (s.k0 + s.j * BT);
-    // a wait that ran out leaves the loops running on whatever is there: the error word tells
-    mbar_wait_err(bar_full + 8 * st, (k / C::ST) & 1, abort_flag, &g_shared_prefix_error, kErrWait);
-    const int key0 = kq * (BT / wk);
-    if (wm * 16 < s.rn && key0 < nvalid) {
-      if (wk == 1) {
-        if (nvalid >= BT) w.template tile<1, false>(sk, sv, 0, BT);
-        else w.template tile<1, true>(sk, sv, 0, nvalid);
-      } else if (wk == 2) {
-        if (nvalid >= BT) w.template tile<2, false>(sk, sv, key0, BT);
-        else w.template tile<2, true>(sk, sv, key0, nvalid);
-      } else {
-        if (nvalid >= BT) w.template tile<4, false>(sk, sv, key0, BT);
-        else w.template tile<4, true>(sk, sv, key0, nvalid);
-      }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar_empty + 8 * st);
-    Cursor e = s;
-    const bool more = s.next(unit, a.units, a.nkv);
-    if (more && x + 1 < x1) continue;
-    // end of the segment e: join the warps that split its keys, then leave the partial
-    w.finish_sums();
-    for (int step = wk / 2; step > 0; step /= 2)
-      for (int h = 0; h < 2; ++h) {
-        if (h == 1 && e.rn <= 8) break;
-        float* buf = red + (wk == 4 ? kq % step : wm) * (HD / 4 + 2) * 32;
-        if (kq >= step && kq < 2 * step) w.put(buf, h);
-        consumers_sync();
-        if (kq < step) w.join(buf, h);
-        consumers_sync();
-      }
-    if (kq == 0) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int rl = wm * 16 + w.g + 8 * h;
-        if (rl < e.rn) {
-          long long slot;
-          if (j0 == 0) {  // the unit's first segment: a slot of the row; another one: a slot of the CTA
-            const int r = e.r0 + rl;
-            slot = (long long)(e.row0 + r / a.Gq) * a.nq + e.kvh * a.Gq + r % a.Gq;
-            if (e.u >= a.units - a.B) slot += nqt;
+      const Cursor e = s;
+      const int wk = e.rn <= 16 ? 4 : e.rn <= 32 ? 2 : 1;
+      const int wm = warp / wk, kq = warp % wk, key0 = kq * (BT / wk);
+      w.start(a, e, wm);
+      for (bool more = true; more; ++k) {
+        const int st = k % ST;
+        const uint32_t sk = base + st * 2 * C::BYTES, sv = sk + C::BYTES;
+        const int nvalid = e.k1 - (e.k0 + s.j * BT);
+        more = s.next();
+        // a wait that ran out leaves the loops running on whatever is there: the error word tells
+        mbar_wait_err(bar_full + 8 * st, (k / ST) & 1, abort_flag, &g_shared_prefix_error, kErrWait);
+        if (wm * 16 < e.rn && key0 < nvalid) {
+          if (wk == 1) {
+            if (nvalid >= BT) w.template tile<BT, false>(sk, sv, 0, BT);
+            else w.template tile<BT, true>(sk, sv, 0, nvalid);
+          } else if (wk == 2) {
+            if (nvalid >= BT) w.template tile<BT / 2, false>(sk, sv, key0, BT);
+            else w.template tile<BT / 2, true>(sk, sv, key0, nvalid);
           } else {
-            slot = 2LL * nqt + (long long)blockIdx.x * MR + rl;
+            if (nvalid >= BT) w.template tile<BT / 4, false>(sk, sv, key0, BT);
+            else w.template tile<BT / 4, true>(sk, sv, key0, nvalid);
           }
-          w.store(a.part_o + slot * HD, a.part_ml + slot * 2, h);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_empty + 8 * st);
+      }
+      join_warps(w, red, (HD / 4 + 2) * 32, wk, wm, kq, e.rn);
+      if (kq == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int rl = wm * 16 + w.g + 8 * h;
+          if (rl < e.rn) {
+            const long long slot = partial_slot(a, e, line, 0, rl);
+            w.store(a.part_o + slot * HD, a.part_ml + slot * 2, h);
+          }
         }
       }
     }
-    first = true;
   }
+}
+
+// ------------------------------------------------------------------ tcgen05 variant
+// One CTA per SM, 128 keys at a time, keys on the M side of both products:
+//
+//   S_j = K_j Q^T       M 128 keys, N query rows (16, 32 or 64), K HD
+//   O  += V_j^T P_j     M dims (twice the same 64 for HD 64), N query rows, K 128 keys
+//
+// so that a suffix unit with a handful of query rows costs a handful of columns, and a softmax thread
+// owns a key: N exponentials per 128 keys.  Decode is bound by the cache's bytes, and this keeps the work
+// per byte low on both kinds of units.
+//
+// The chain from S to P is latency, not work, so two groups of four softmax warps take turns: tile by
+// tile, each with its own maxima, sums, P and O.  The even and the odd tiles of a segment are two
+// partials for the combine kernel.
+//
+// P = 2^(S - m) needs no maximum for its precision, only a range: m is the score of a segment's first
+// key (of the group's first tile), one per query row, so the largest P is at least 1.  bf16 has the exponents
+// of fp32, so P may reach 2^60; f16 2^15.  A barrier's OR tells when a value exceeds that; only then are
+// maxima taken (warp reductions, then across the four warps), O and the sums rescaled and P formed again.
+//
+// A segment's O is stored when the group's next tile waits for the same product anyway.
+//
+// warp 0       loads K and V tiles (TMA) into a ring of entries, K and V apart
+// warp 1       issues the products, S up to two tiles ahead (of the next unit, too)
+// warp 2       brings the query rows of the next segments to shared memory
+// warps 4-11   softmax: thread r of a group owns key r of its tiles, and dim r of its output
+// warps 12-15  (e4m3 cache) convert tiles to f16, which holds e4m3 values exactly
+template <int HD, bool F8>
+struct Tc {
+  using E = Tile<HD, false, 128>;  // K or V as the products read it (2-byte type)
+  using R = Tile<HD, F8, 128>;     // as the cache holds it
+  static constexpr int THREADS = F8 ? 512 : 384;
+  static constexpr int Q = (MR + 16) * HD * 2;  // see QPlace
+  static constexpr int P = 128 * MR * 2;
+  // places for K and V tiles as the products read them, and for raw ones.  K and V have rings of their own:
+  // a K tile is free as soon as its S is complete, a V tile only after P, and in one ring it would hold up the
+  // K tiles behind it.
+  static constexpr int KN = F8 ? (HD == 128 ? 1 : 2) : (HD == 128 ? 2 : 4);
+  static constexpr int VN = F8 ? (HD == 128 ? 2 : 3) : (HD == 128 ? 3 : 6);
+  static constexpr int RN = F8 ? (HD == 128 ? 4 : 8) : 0;
+  static constexpr int QB = 5;                     // query buffers: one for the prefix line, up to 4 for the suffix line
+  static constexpr int BARS = 2 * (KN + VN + RN) + 2 * QB + 4 + 4;
+  static constexpr int STAT = 2 * MR * 8 + (4 + 2 + 1 + 1) * MR * 4;  // of a softmax group, see Stat
+  static constexpr int SMEM =
+      1024 + Q + 2 * P + (KN + VN) * E::BYTES + RN * R::BYTES + 2 * STAT + (MR + 16) * 4 + BARS * 8 + 16;
+  static constexpr uint32_t COLS = 512;  // tensor memory: S four times 64, O twice 64
+  static constexpr uint32_t FMT = (1u << 4) | (8u << 24) | (F8 ? 0u : (1u << 7) | (1u << 10));  // M 128, f16 or bf16
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+// Shared-memory matrix descriptors (128-byte swizzle, 8-row groups 1024 bytes apart) in two words: the low
+// one is the address / 16, with the leading offset / 16 above it, and advances by plain additions; the high one
+// is the same for all.  The issuing thread has a few hundred cycles for the 16 products of a tile, so
+// nothing but additions is left to it.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t leading) { return (saddr >> 4) | ((leading >> 4) << 16); }
+template <bool ACC>
+__device__ __forceinline__ void umma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc = 1) {
+  if constexpr (ACC)
+    asm volatile(
+        "{\n .reg .b64 x, y;\n .reg .pred p;\n mov.b64 x, {%1, %4};\n mov.b64 y, {%2, %4};\n setp.eq.u32 p, 0, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(tmem_d),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(kDescHi));
+  else
+    asm volatile(
+        "{\n .reg .b64 x, y;\n .reg .pred p;\n mov.b64 x, {%1, %4};\n mov.b64 y, {%2, %4};\n setp.ne.u32 p, %5, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(tmem_d),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(kDescHi), "r"(acc));
+}
+// n columns of this thread's lane, complete on return (one statement: nothing can use them before)
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float* r);
+template <>
+__device__ __forceinline__ void tmem_load<16>(uint32_t taddr, float* r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      " tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(taddr)
+      : "memory");
+}
+template <>
+__device__ __forceinline__ void tmem_load<32>(uint32_t taddr, float* r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      " tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* r) {
+  const uint32_t* u = reinterpret_cast<const uint32_t*>(r);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(
+          taddr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+      : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+// barriers of softmax group wg: 1 + 2 wg, and 2 + 2 wg for the OR of a predicate
+__device__ __forceinline__ void group_sync(int wg) { asm volatile("bar.sync %0, 128;\n" ::"r"(1 + 2 * wg) : "memory"); }
+__device__ __forceinline__ bool group_any(int wg, bool x) {
+  int r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 q, %1, 0;\n barrier.cta.red.or.pred p, %2, 128, q;\n selp.s32 %0, 1, 0, p;\n}\n"
+      : "=r"(r)
+      : "r"((int)x), "r"(2 + 2 * wg)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ float warp_max_f32(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;\n" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// A CTA's tiles in order: its run of the prefix line, then its run of the suffix line.
+struct Walk {
+  Cursor s;
+  int line, seg, t;  // segments of the line so far, tiles of the segment so far
+  bool valid;
+  __device__ __forceinline__ void begin(const Args& a) {
+    seg = t = line = 0;
+    valid = s.begin(a, 0);
+    if (!valid) {
+      line = 1;
+      valid = s.begin(a, 1);
+    }
+  }
+  __device__ __forceinline__ bool last_of_segment() const { return s.j + 1 == s.n || s.x + 1 == s.x1; }
+  // to the next tile; true when it belongs to the same segment
+  __device__ __forceinline__ bool next(const Args& a) {
+    ++t;
+    if (s.next()) return true;
+    ++seg;
+    t = 0;
+    if (s.done()) {
+      valid = line == 0 && s.begin(a, 1);
+      line = 1;
+      seg = 0;
+    }
+    return false;
+  }
+};
+// columns of a segment with rn query rows
+__device__ __forceinline__ int columns(int rn) { return rn <= 16 ? 16 : rn <= 32 ? 32 : 64; }
+
+// The place of a segment's query rows: the first MR rows of the buffer for the prefix line; for the suffix
+// line 1, 2 or 4 places, of which the first lies behind them where it fits (so the line's first rows need
+// not wait for the prefix line's last product).  Each place has its own pair of barriers.
+struct QPlace {
+  int bar, row0, rows;  // barrier pair, first row in the buffer (a multiple of 8), rows of a span
+  uint32_t parity;
+  bool shared;  // lies in the prefix line's rows
+  __device__ __forceinline__ QPlace(const Args& a, int line, int seg) {
+    rows = line ? columns(a.Gq) : MR;
+    const int lg = rows == 64 ? 0 : rows == 32 ? 1 : 2, i = seg & ((1 << lg) - 1);
+    bar = line ? 1 + i : 0;
+    shared = !(rows == 16 && i == 0);
+    row0 = shared ? i * rows : MR;
+    parity = (seg >> lg) & 1;
+  }
+};
+
+constexpr float kNoMax = -1e30f;  // where a row has no score yet: every score exceeds it by far
+
+// what the threads of a softmax group share
+struct Stat {
+  long long* slot;  // [2][MR] where the partials go, of a segment and of the one before
+  float* red;       // [4][MR] per warp: maxima, sums
+  float* m;         // [2][MR] reference scores in use (log2)
+  float* alpha;     // [MR]
+  float* c;         // [MR] score factors of the query rows (e4m3 cache)
+};
+__device__ __forceinline__ void load4(float* d, const float* s) {
+  const float4 v = *reinterpret_cast<const float4*>(s);
+  d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+}
+
+template <int HD, bool F8, int N>
+struct Softmax {
+  static constexpr int H = N < 32 ? N : 32;  // columns at a time
+  static constexpr float kMost = F8 ? 32768.f : 1152921504606846976.f;  // 2^15, 2^60
+
+  // 2^(S - m) of this thread's key, packed, and the largest of them
+  static __device__ __forceinline__ float weights(uint32_t* p, uint32_t t_s, bool live, float scale, const float* sm,
+                                                  const float* sc) {
+    float top = 0.f;
+#pragma unroll
+    for (int h = 0; h < N; h += H) {
+      float y[H];
+      tmem_load<H>(t_s + h, y);
+#pragma unroll
+      for (int i = 0; i < H; i += 4) {
+        float m[4], c[4];
+        load4(m, sm + h + i);
+        if (F8) load4(c, sc + h + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[i + e] = ex2(y[i + e] * (F8 ? c[e] : scale) - m[e]);
+          top = fmaxf(top, y[i + e]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < H; i += 2) {
+        const uint32_t v = F8 ? pack_f16(y[i], y[i + 1]) : pack_bf16(y[i], y[i + 1]);
+        p[(h + i) / 2] = live ? v : 0u;
+      }
+    }
+    return live ? top : 0.f;
+  }
+
+  // the scores of the tile's first key, which is always one of the row's (thread 0)
+  static __device__ __forceinline__ void refer(uint32_t t_s, float scale, float* sm, const float* sc) {
+#pragma unroll
+    for (int h = 0; h < N; h += 16) {
+      float y[16];
+      tmem_load<16>(t_s + h, y);
+      if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = y[i] * (F8 ? sc[h + i] : scale);
+          sm[h + i] = x == -INFINITY ? kNoMax : x;
+        }
+    }
+  }
+
+  // one tile up to P (packed in p) and the sums of the rounded P in l; wait_o() waits for the group's
+  // product before
+  template <typename W>
+  static __device__ __forceinline__ void tile(int wg, uint32_t t_s, uint32_t t_o, bool live, bool first, float scale,
+                                              const Stat& st, float* sm, float* l, uint32_t* p, int r, W wait_o) {
+    const int warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+    if (first) {
+      if (warp4 == 0) refer(t_s, scale, sm, st.c);
+      group_sync(wg);
+    }
+    if (group_any(wg, weights(p, t_s, live, scale, sm, st.c) > kMost)) {
+#pragma unroll
+      for (int h = 0; h < N; h += H) {
+        float y[H];
+        tmem_load<H>(t_s + h, y);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          const float mx = warp_max_f32(live ? y[i] * (F8 ? st.c[h + i] : scale) : -INFINITY);
+          if (lane == i) st.red[warp4 * MR + h + i] = mx;
+        }
+      }
+      group_sync(wg);
+      if (r < N) {
+        const float old = sm[r];
+        const float mx = fmaxf(fmaxf(st.red[r], st.red[MR + r]), fmaxf(st.red[2 * MR + r], st.red[3 * MR + r]));
+        const float now = fmaxf(old, mx);
+        st.alpha[r] = ex2(old - now);
+        sm[r] = now;
+      }
+      group_sync(wg);
+      if (!first) {
+        wait_o();
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < N; h += 16) {
+          float o[16];
+          tmem_load<16>(t_o + h, o);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float f = st.alpha[h + i];
+            o[i] *= f;
+            l[h + i] *= f;
+          }
+          tmem_st16(t_o + h, o);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+      }
+      weights(p, t_s, live, scale, sm, st.c);
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 v = F8 ? __half22float2(*reinterpret_cast<__half2*>(&p[i]))
+                          : __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&p[i]));
+      l[2 * i] += v.x;
+      l[2 * i + 1] += v.y;
+    }
+  }
+
+  static __device__ __forceinline__ void write(const uint32_t* p, uint8_t* prow, int r) {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i)
+      *reinterpret_cast<uint4*>(prow + ((i ^ (r & 7)) << 4)) = make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
+  }
+
+  // sums of l over the warp's 32 keys, each column once: exchanges of ever smaller halves
+  static __device__ __forceinline__ void reduce(float* l, float* red) {
+    const int warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+    int n = N;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const bool up = lane & o;
+      if (n > 1) {
+        n /= 2;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+          if (i < n) {
+            const float send = up ? l[i] : l[i + n], keep = up ? l[i + n] : l[i];
+            l[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+          }
+      } else {
+        l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+      }
+    }
+    if constexpr (N == 64) {
+      red[warp4 * MR + 2 * lane] = l[0];
+      red[warp4 * MR + 2 * lane + 1] = l[1];
+    } else {
+      red[warp4 * MR + lane / (32 / N)] = l[0];
+    }
+  }
+
+};
+
+// a segment's outputs: thread r has dim r
+template <int HD>
+__device__ __forceinline__ void store_o(uint32_t t_o, const long long* slot, float* part_o, int rn, int r) {
+  for (int h = 0; h < rn; h += 16) {
+    float o[16];
+    tmem_load<16>(t_o + h, o);
+    if (r < HD)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (h + i < rn) part_o[slot[h + i] * HD + r] = o[i];
+  }
+}
+
+template <int HD, bool F8>
+__global__ void __launch_bounds__(Tc<HD, F8>::THREADS, 1)
+shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                        const __grid_constant__ Args a) {
+  using T = Tc<HD, F8>;
+  using E = typename T::E;
+  using R = typename T::R;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t s_q = base;                           // query rows
+  const uint32_t s_p = s_q + T::Q;                     // [2] P of the softmax groups
+  const uint32_t s_k = s_p + 2 * T::P;                 // [KN]
+  const uint32_t s_v = s_k + T::KN * E::BYTES;         // [VN]
+  const uint32_t s_r = s_v + T::VN * E::BYTES;         // [RN]
+  uint8_t* g_stat = gbase + (s_r - base) + T::RN * R::BYTES;
+  float* q_factor = reinterpret_cast<float*>(g_stat + 2 * T::STAT);  // of the rows of the query buffer
+  uint64_t* bars = reinterpret_cast<uint64_t*>(q_factor + MR + 16);
+  const uint32_t bar_k = smem_u32(bars);               // [KN] K ready for the products
+  const uint32_t bar_kfree = bar_k + 8 * T::KN;        // [KN] K read
+  const uint32_t bar_v = bar_kfree + 8 * T::KN;        // [VN] V ready
+  const uint32_t bar_vfree = bar_v + 8 * T::VN;        // [VN] V read
+  const uint32_t bar_r = bar_vfree + 8 * T::VN;        // [RN] raw tile landed
+  const uint32_t bar_rfree = bar_r + 8 * T::RN;        // [RN] raw tile converted
+  const uint32_t bar_q = bar_rfree + 8 * T::RN;        // [QB] query rows ready
+  const uint32_t bar_qfree = bar_q + 8 * T::QB;        // [QB] query rows (and factors) read
+  const uint32_t bar_s = bar_qfree + 8 * T::QB;        // [4] S complete
+  const uint32_t bar_p = bar_s + 32;                   // [2] S read, P written, O rescaled
+  const uint32_t bar_o = bar_p + 16;                   // [2] O complete up to the tile
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + T::BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    return mbar_wait_err(bar, parity, abort_flag, &g_shared_prefix_error, kErrWait);
+  };
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < T::KN; ++i) {
+      mbar_init(bar_k + 8 * i, F8 ? 4 : 1);
+      mbar_init(bar_kfree + 8 * i, 1);
+    }
+    for (int i = 0; i < T::VN; ++i) {
+      mbar_init(bar_v + 8 * i, F8 ? 4 : 1);
+      mbar_init(bar_vfree + 8 * i, 1);
+    }
+    for (int i = 0; i < T::RN; ++i) {
+      mbar_init(bar_r + 8 * i, 1);
+      mbar_init(bar_rfree + 8 * i, 4);
+    }
+    for (int i = 0; i < T::QB; ++i) {
+      mbar_init(bar_q + 8 * i, 2);
+      mbar_init(bar_qfree + 8 * i, F8 ? 3 : 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar_s + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_p + 8 * i, 4);
+      mbar_init(bar_o + 8 * i, 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)),
+                 "r"(T::COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, t_o = tmem + 4 * MR;
+  pdl_wait();
+  // the walk is the same in every role: tile k belongs to softmax group k & 1.  Tiles are loaded in the order
+  // K_0, K_1, V_0, K_2, V_1, ...
+  // (e4m3) 512 threads start with 128 registers each; the softmax groups take over what the others do not
+  // need: 2 x 80 + 2 x 168 = 496 of 4 x 128
+  if (warp < 4) {
+  if constexpr (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
+  if (warp == 0) {
+    Feed fk, fv;
+    int nk = 0, nv = 0;
+    auto put = [&](auto is_v) {  // the next K or V tile to its place
+      constexpr int kv = decltype(is_v)::value, n = F8 ? T::RN : kv ? T::VN : T::KN;
+      Feed& d = kv ? fv : fk;
+      const int i = F8 ? nk + nv : kv ? nv : nk, at = i % n;
+      const uint32_t full = (F8 ? bar_r : kv ? bar_v : bar_k) + 8 * at;
+      const uint32_t free = (F8 ? bar_rfree : kv ? bar_vfree : bar_kfree) + 8 * at;
+      const uint32_t dst = (F8 ? s_r : kv ? s_v : s_k) + at * R::BYTES;
+      if (!wait(free, ((i / n) & 1) ^ 1)) return false;
+      if (elect_one()) mbar_expect_tx(full, d.template bytes<R>(a.box));
+      __syncwarp();
+      d.template load<R>(a, kv ? &tv : &tk, a.box, dst, full);
+      ++(kv ? nv : nk);
+      d.next(a, 128);
+      return true;
+    };
+    const std::integral_constant<int, 0> k_tile;
+    const std::integral_constant<int, 1> v_tile;
+    fk.begin(a, 128);
+    fv.begin(a, 128);
+    bool ok = !fk.valid || put(k_tile);
+    while (ok && fv.valid) ok = (!fk.valid || put(k_tile)) && put(v_tile);
+    if (__any_sync(0xffffffffu, *abort_flag)) {
+      if constexpr (F8) {
+        drain(bar_r, T::RN, nk + nv);
+      } else {
+        drain(bar_k, T::KN, nk);
+        drain(bar_v, T::VN, nv);
+      }
+    }
+  } else if (warp == 1) {
+    Walk w;
+    w.begin(a);
+    int ka = 0;                      // tiles whose S is issued
+    int ki = 0, vi = 0;              // places of the next K and V
+    uint32_t kph = 0, vph = 0;
+    uint32_t info = 0;               // of tile i, at bits 8 (i & 3): columns / 8, and 16 when O is added to
+    QPlace q(a, w.line, w.seg);
+    auto issue_s = [&] {
+      if (w.t == 0) {
+        q = QPlace(a, w.line, w.seg);
+        if (!wait(bar_q + 8 * q.bar, q.parity)) return false;
+      }
+      // the buffer of S is free: P of tile ka - 4 was awaited
+      if (!wait(bar_k + 8 * ki, kph)) return false;
+      tc_fence_after();
+      const int sb = ka & 3;
+      const uint32_t n8 = columns(w.s.rn) >> 3, id = T::FMT | (n8 << 17);
+      const uint32_t kd = desc_lo(s_k + ki * E::BYTES, 0), qd = desc_lo(s_q + q.row0 * (HD * 2), 0);
+      const uint32_t span = (uint32_t)q.rows * 8;  // 128 bytes a row, in units of 16
+      const bool last = w.last_of_segment();
+      if (elect_one()) {
+        umma<false>(tmem + sb * MR, kd, qd, id, 0);
+#pragma unroll
+        for (int kk = 1; kk < HD / 16; ++kk)
+          umma<true>(tmem + sb * MR, kd + (kk >> 2) * 1024 + (kk & 3) * 2, qd + (kk >> 2) * span + (kk & 3) * 2, id);
+        umma_commit(bar_s + 8 * sb);
+        umma_commit(bar_kfree + 8 * ki);
+        if (last) umma_commit(bar_qfree + 8 * q.bar);
+      }
+      __syncwarp();
+      info = (info & ~(0xffu << (8 * sb))) | ((n8 | (w.t >= 2 ? 16u : 0u)) << (8 * sb));
+      w.next(a);
+      ++ka;
+      if (++ki == T::KN) ki = 0, kph ^= 1;
+      return true;
+    };
+    bool ok = true;
+    while (ok && w.valid && ka < 2) ok = issue_s();
+    for (int k = 0; ok && k < ka; ++k) {
+      const int wg = k & 1;
+      ok = wait(bar_v + 8 * vi, vph) && wait(bar_p + 8 * wg, (k >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t i = info >> (8 * (k & 3)), id = T::FMT | (1u << 15) | (1u << 16) | ((i & 15u) << 17);
+      const uint32_t vd = desc_lo(s_v + vi * E::BYTES, HD == 128 ? 128 * 128 : 0), pd = desc_lo(s_p + wg * T::P, 0);
+      if (elect_one()) {
+        umma<false>(t_o + wg * MR, vd, pd, id, i & 16u);
+#pragma unroll
+        for (int kk = 1; kk < 8; ++kk) umma<true>(t_o + wg * MR, vd + kk * 128, pd + kk * 128, id);
+        umma_commit(bar_o + 8 * wg);
+        umma_commit(bar_vfree + 8 * vi);
+      }
+      __syncwarp();
+      if (++vi == T::VN) vi = 0, vph ^= 1;
+      if (w.valid) ok = issue_s();
+    }
+  } else {
+    // query rows, half of them a warp: LPR lanes a row, 16 bytes each; rows up to the segment's columns are zero
+    constexpr int LPR = HD / 8, RPI = 64 / LPR;
+    const int ch = lane % LPR, first_row = (warp - 2) * (32 / LPR) + lane / LPR;
+    Walk w;
+    int prefix_segs = 0;
+    for (w.begin(a); w.valid;) {
+      const QPlace q(a, w.line, w.seg);
+      if (!wait(bar_qfree + 8 * q.bar, q.parity ^ 1)) break;
+      if (w.line == 0) {
+        ++prefix_segs;
+      } else if (prefix_segs > 0 && q.shared) {  // the prefix line's products have read its rows
+        if (!wait(bar_qfree, (prefix_segs - 1) & 1)) break;
+        prefix_segs = 0;
+      }
+      const int rows = columns(w.s.rn);
+      auto src = [&](int r) {
+        const uint32_t rr = w.s.r0 + r, b = a.Gq == 1 ? rr : __umulhi(rr, a.inv_gq), h = rr - b * a.Gq;
+        return a.q + (long long)(w.s.row0 + b) * a.q_row + (long long)(w.s.kvh * a.Gq + h) * a.q_head + ch * 8;
+      };
+      const uint32_t at = q.row0 * (HD * 2) + (ch >> 3) * (q.rows * 128);
+      if constexpr (!F8) {
+        for (int r = first_row; r < rows; r += RPI)
+          cp_async16_or_zero(s_q + at + r * 128 + (((ch & 7) ^ (r & 7)) << 4), r < w.s.rn ? src(r) : a.q, r < w.s.rn);
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
+      } else {
+        constexpr int U = 4;  // rows in flight a lane
+        for (int r0 = first_row; r0 < rows; r0 += U * RPI) {
+          uint4 v[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            v[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (r0 + u * RPI < w.s.rn) v[u] = *reinterpret_cast<const uint4*>(src(r0 + u * RPI));
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * RPI;
+            uint32_t* x = reinterpret_cast<uint32_t*>(&v[u]);
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x[i]));
+              mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const int ex = f16_row_exponent(mx);
+            const float f = f16_row_factor(ex);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 g = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x[i]));
+              x[i] = pack_f16(g.x * f, g.y * f);
+            }
+            if (r < rows) {
+              if (ch == 0) q_factor[q.row0 + r] = a.scale_log2 * f16_row_inverse(ex);
+              *reinterpret_cast<uint4*>(gbase + at + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v[u];
+            }
+          }
+        }
+      }
+      fence_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q + 8 * q.bar);
+      while (w.next(a)) {
+      }
+    }
+  }
+  } else if (warp < 12) {
+    if constexpr (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
+    // every thread takes every step whatever its waits say (the error word tells): the barriers stay in step
+    const int wg = (warp >> 2) - 1, r = threadIdx.x & 127;  // key of a tile, dim of the output
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16, t_og = t_o + lane_off + wg * MR;
+    uint8_t* prow = gbase + (s_p - base) + wg * T::P + r * 128;
+    Stat st;
+    st.slot = reinterpret_cast<long long*>(g_stat + wg * T::STAT);
+    st.red = reinterpret_cast<float*>(st.slot + 2 * MR);
+    st.m = st.red + 4 * MR;
+    st.alpha = st.m + 2 * MR;
+    st.c = st.alpha + MR;
+    Walk w;
+    int k = 0, mine = 0, buf = 0, left = 0;  // the group's tiles, segments mod 2, query rows whose O is not stored yet
+    auto wait_o = [&] {  // the group's product before
+      if (mine > 0) wait(bar_o + 8 * wg, (mine - 1) & 1);
+    };
+    auto flush = [&] {  // the O of the segment before
+      if (left > 0) store_o<HD>(t_og, st.slot + (buf ^ 1) * MR, a.part_o, left, r);
+      left = 0;
+    };
+    for (w.begin(a); w.valid;) {
+      const Cursor s = w.s;
+      const bool mine0 = (k & 1) == wg;               // the segment's first tile is this group's
+      const bool part = mine0 || !w.last_of_segment();  // the segment has a tile of this group
+      if (part && r < s.rn) st.slot[buf * MR + r] = partial_slot(a, s, w.line, mine0 ? 0 : 1, r);
+      if constexpr (F8) {
+        const QPlace q(a, w.line, w.seg);
+        wait(bar_q + 8 * q.bar, q.parity);
+        if (r < q.rows) st.c[r] = q_factor[q.row0 + r];
+        group_sync(wg);
+        if (r == 0) mbar_arrive(bar_qfree + 8 * q.bar);
+      }
+      float l[MR];
+#pragma unroll
+      for (int i = 0; i < MR; ++i) l[i] = 0.f;
+      float* sm = st.m + buf * MR;
+      bool first = true;
+      for (bool same = true; same; ++k) {
+        const int nvalid = s.k1 - (s.k0 + w.s.j * 128);
+        same = w.next(a);
+        if ((k & 1) != wg) continue;
+        const bool live = r < nvalid;
+        const int sb = k & 3;
+        wait(bar_s + 8 * sb, (k >> 2) & 1);
+        tc_fence_after();
+        const uint32_t t_s = tmem + lane_off + sb * MR;
+        uint32_t p[MR / 2];
+        if (s.rn <= 16) Softmax<HD, F8, 16>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
+        else if (s.rn <= 32) Softmax<HD, F8, 32>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
+        else Softmax<HD, F8, 64>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
+        wait_o();  // it reads P's place
+        tc_fence_after();
+        if (first) flush();
+        first = false;
+        if (s.rn <= 16) Softmax<HD, F8, 16>::write(p, prow, r);
+        else if (s.rn <= 32) Softmax<HD, F8, 32>::write(p, prow, r);
+        else Softmax<HD, F8, 64>::write(p, prow, r);
+        if (nvalid < 128) {  // what lies behind the last key may be anything: P is 0 there, and V must be finite
+          const int e = k % T::VN;
+          wait(bar_v + 8 * e, (k / T::VN) & 1);
+          if (!live)
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i)
+              *reinterpret_cast<uint4*>(gbase + (s_v - base) + e * E::BYTES + E::at(r, i)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_async();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p + 8 * wg);
+        ++mine;
+      }
+      if (part) {
+        if (s.rn <= 16) Softmax<HD, F8, 16>::reduce(l, st.red);
+        else if (s.rn <= 32) Softmax<HD, F8, 32>::reduce(l, st.red);
+        else Softmax<HD, F8, 64>::reduce(l, st.red);
+        group_sync(wg);
+        if (r < s.rn) {
+          const float m = sm[r] == kNoMax ? -INFINITY : sm[r];
+          const float sum = (st.red[r] + st.red[MR + r]) + (st.red[2 * MR + r] + st.red[3 * MR + r]);
+          *reinterpret_cast<float2*>(a.part_ml + st.slot[buf * MR + r] * 2) = make_float2(m, sum);
+        }
+        left = s.rn;
+        buf ^= 1;
+      }
+    }
+    wait_o();
+    tc_fence_after();
+    flush();
+  } else if constexpr (F8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
+    const int tid = threadIdx.x - 384;
+    constexpr int CH = HD / 16;  // chunks of 16 values of a key
+    Cursor s;
+    int tiles = 0;
+    for (int line = 0; line < 2; ++line)
+      if (s.begin(a, line)) tiles += s.x1 - s.x;
+    int nk = 0, nv = 0;
+    for (int e = 0; e < 2 * tiles; ++e) {
+      const bool is_k = e == 0 || ((e & 1) && nk < tiles);  // the order of the loads
+      const int ri = e % T::RN, i = is_k ? nk % T::KN : nv % T::VN;
+      const uint32_t full = (is_k ? bar_k : bar_v) + 8 * i, free = (is_k ? bar_kfree : bar_vfree) + 8 * i;
+      if (!wait(bar_r + 8 * ri, (e / T::RN) & 1) || !wait(free, ((is_k ? nk / T::KN : nv / T::VN) & 1) ^ 1)) break;
+      ++(is_k ? nk : nv);
+      const uint8_t* src = gbase + (s_r - base) + ri * R::BYTES;
+      uint8_t* dst = gbase + ((is_k ? s_k : s_v) - base) + i * E::BYTES;
+#pragma unroll 4
+      for (int x = tid; x < 128 * CH; x += 128) {
+        // 4 chunks of 8 rows a warp: the stores of a quarter warp meet no bank twice
+        const int ch = (x & 3) + 4 * (x / 512), row = (x >> 2) & 127;
+        const uint4 v = *reinterpret_cast<const uint4*>(src + R::at(row, ch));
+        *reinterpret_cast<uint4*>(dst + E::at(row, 2 * ch)) =
+            make_uint4(e4m3x2_f16x2(v.x), e4m3x2_f16x2(v.x >> 16), e4m3x2_f16x2(v.y), e4m3x2_f16x2(v.y >> 16));
+        *reinterpret_cast<uint4*>(dst + E::at(row, 2 * ch + 1)) =
+            make_uint4(e4m3x2_f16x2(v.z), e4m3x2_f16x2(v.z >> 16), e4m3x2_f16x2(v.w), e4m3x2_f16x2(v.w >> 16));
+      }
+      fence_async();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(full);
+        mbar_arrive(bar_rfree + 8 * ri);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(T::COLS));
 }
 
 // ----------------------------------------------------------------------- combine
@@ -755,7 +1538,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
 // order of the keys.
 template <int HD>
 __global__ void __launch_bounds__(128)
-shared_prefix_combine_kernel(const int* __restrict__ plan, int ctas, int units, int B, int nq, int nkv, int Gq,
+shared_prefix_combine_kernel(const int* __restrict__ plan, int ctas, int subs, int units, int B, int nq, int nkv, int Gq,
                              const float* __restrict__ part_o, const float* __restrict__ part_ml, float v_scale,
                              bf16* __restrict__ out) {
   constexpr int V = HD / 32;
@@ -764,8 +1547,7 @@ shared_prefix_combine_kernel(const int* __restrict__ plan, int ctas, int units, 
   const int i = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (i >= B * nq) return;
   const int b = i / nq, h = i - b * nq, kvh = h / Gq, hl = h - kvh * Gq;
-  const int per = plan[0];
-  const int* unit = plan + kHeader + ctas;
+  const int* unit = plan + unit_offset(ctas);
   const int* row = unit + units * kUnitInts + b * kRowInts;
   const int nqt = B * nq;
   float M = -INFINITY, L = 0.f, o[V];
@@ -784,19 +1566,24 @@ shared_prefix_combine_kernel(const int* __restrict__ plan, int ctas, int units, 
 #pragma unroll
     for (int d = 0; d < V; ++d) o[d] = o[d] * fa + p[d] * fb;
   };
-  auto add_unit = [&](int u, int local, long long first_slot) {
-    const int n = unit[u * kUnitInts + 1];
+  auto add_unit = [&](int line, int u, int local) {
+    const int n = unit[u * kUnitInts + 1], per = plan[2 * line];
     if (n == 0) return;
     const int x = unit[u * kUnitInts] * nkv + kvh * n;
-    add(first_slot);
-    for (int c = x / per + 1; c <= (x + n - 1) / per; ++c) add(2LL * nqt + (long long)c * MR + local);
+    for (int c = x / per; c <= (x + n - 1) / per; ++c) {
+      const int tiles = min(x + n, (c + 1) * per) - max(x, c * per);
+      for (int sub = 0; sub < min(subs, tiles); ++sub) {
+        const int ls = 2 * line + sub;
+        add(c * per <= x ? (long long)ls * nqt + i : 4LL * nqt + ((long long)ls * ctas + c) * MR + local);
+      }
+    }
   };
   if (row[2]) {  // a row without keys stays zero
     if (row[0] >= 0) {
       const int r = (b - row[1]) * Gq + hl;
-      add_unit(row[0] + r / MR, r % MR, i);
+      add_unit(0, row[0] + r / MR, r % MR);
     }
-    add_unit(units - B + b, hl, (long long)nqt + i);
+    add_unit(1, units - B + b, hl);
   }
   const float inv = L == 0.f ? 0.f : v_scale / L;
   bf16* po = out + (long long)i * HD + lane * V;
@@ -804,27 +1591,34 @@ shared_prefix_combine_kernel(const int* __restrict__ plan, int ctas, int units, 
   for (int d = 0; d < V; ++d) po[d] = __float2bfloat16_rn(o[d] * inv);
 }
 
-// 3-D map of a cache: [pages * block keys][KV heads][dims], boxes of `box` keys of one head
-CUtensorMap cache_tmap(const at::Tensor& c, int box, bool f8) {
+// 4-D map of a cache: [128-byte spans of a key][pages * block keys][KV heads][dims of a span], boxes of
+// `box` keys of one head; a box of `whole` keys brings every span
+CUtensorMap cache_tmap(const at::Tensor& c, int box, int whole, bool f8) {
   CUtensorMap m;
   const int hd = c.size(3), nkv = c.size(2), elt = f8 ? 1 : 2;
-  const int inner = std::min(hd * elt, 128);
-  cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)nkv, (cuuint64_t)(c.size(0) * c.size(1))};
-  cuuint64_t strides[2] = {(cuuint64_t)hd * elt, (cuuint64_t)nkv * hd * elt};
-  cuuint32_t bx[3] = {(cuuint32_t)(inner / elt), 1u, (cuuint32_t)box};
-  cuuint32_t estr[3] = {1u, 1u, 1u};
+  const int inner = std::min(hd * elt, 128), spans = hd * elt / inner;
+  cuuint64_t dims[4] = {(cuuint64_t)(inner / elt), (cuuint64_t)nkv, (cuuint64_t)(c.size(0) * c.size(1)), (cuuint64_t)spans};
+  cuuint64_t strides[3] = {(cuuint64_t)hd * elt, (cuuint64_t)nkv * hd * elt, (cuuint64_t)inner};
+  cuuint32_t bx[4] = {(cuuint32_t)(inner / elt), 1u, (cuuint32_t)box, box == whole ? (cuuint32_t)spans : 1u};
+  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
   const CUtensorMapSwizzle sw = inner == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                               : CU_TENSOR_MAP_SWIZZLE_32B;
-  CUresult r = tma_encode_fn()(&m, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+  CUresult r = tma_encode_fn()(&m, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                                c.data_ptr(), dims, strides, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "rl_b200: cuTensorMapEncodeTiled failed (", (int)r, ")");
   return m;
 }
 
-int plan_ints(int ctas, int units, int B) { return kHeader + ctas + units * kUnitInts + B * kRowInts; }
-int grid_ctas() { return 2 * num_sms(); }
+int plan_ints(Shape p, int units, int B) { return unit_offset(p.ctas) + units * kUnitInts + B * kRowInts; }
+
+// keys of a TMA box, at most `most`: a power of two that divides the page, so a box never leaves its
+// page and an aligned stage is whole boxes; 0 below 8 keys (a period of the swizzle)
+int box_keys(int64_t block, int most) {
+  while (block % most) most /= 2;
+  return most < 8 ? 0 : most;
+}
 
 template <typename K, typename... A>
 void launch_pdl(K kern, int grid, int block, int smem, A... args) {
@@ -849,24 +1643,27 @@ using namespace rlb;
 // int32 plan of the work of one decode step (see the kernel): group g's rows are
 // [group_starts[g], group_starts[g+1]), of whose keys the first prefix_lens[g] are the same
 at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, at::Tensor seq_lens, int64_t nq,
-                              int64_t nkv) {
+                              int64_t nkv, int64_t hd, int64_t block) {
   for (const at::Tensor& t : {group_starts, prefix_lens, seq_lens})
     RLB_CHECK(t.is_cuda() && t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous() &&
                   t.device() == seq_lens.device(),
               "shared_prefix_plan: contiguous int32 vectors on one CUDA device expected");
   const int64_t G = prefix_lens.size(0), B = seq_lens.size(0);
   RLB_CHECK(group_starts.size(0) == G + 1, "shared_prefix_plan: group_starts needs one entry more than prefix_lens");
-  RLB_CHECK(nkv >= 1 && nq >= nkv && nq % nkv == 0 && nq / nkv <= sp::MR,
+  RLB_CHECK(nkv >= 1 && nq >= nkv && nq % nkv == 0 && nq / nkv <= sp::kMaxHeads,
             "shared_prefix_plan: query heads must be a multiple of the KV heads, at most 64 per KV head");
-  RLB_CHECK(B <= 8192 && G <= 8192, "shared_prefix_plan: at most 8192 rows and groups");
+  RLB_CHECK(B <= 8192 && G <= 8192 && block >= 1, "shared_prefix_plan: at most 8192 rows and groups");
   const c10::cuda::CUDAGuard guard(seq_lens.device());
-  const int Gq = nq / nkv, ctas = sp::grid_ctas(), units = sp::max_chunks(B, G, Gq) + B;
-  auto plan = at::empty({sp::plan_ints(ctas, units, B)}, seq_lens.options());
-  const int smem = (3 * (int)G + 1 + units) * 4;
+  const int Gq = nq / nkv;
+  const sp::Shape p = sp::shape_of(sp::use_tc(hd, block));
+  const int units = sp::max_chunks(B, G, Gq) + B;
+  auto plan = at::empty({sp::plan_ints(p, units, B)}, seq_lens.options());
+  const int smem = ((int)B + 4 * (int)G + 1 + units) * 4;
   RLB_CHECK(smem <= 200 * 1024, "shared_prefix_plan: too many rows and groups");
-  cudaFuncSetAttribute(sp::shared_prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (smem > 48 * 1024)
+    RLB_CUDA_CHECK(cudaFuncSetAttribute(sp::shared_prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   sp::shared_prefix_plan_kernel<<<1, sp::kPlanThreads, smem, stream()>>>(
-      group_starts.data_ptr<int>(), prefix_lens.data_ptr<int>(), seq_lens.data_ptr<int>(), G, B, Gq, nkv, ctas,
+      group_starts.data_ptr<int>(), prefix_lens.data_ptr<int>(), seq_lens.data_ptr<int>(), G, B, Gq, nkv, p.ctas, p.tile,
       plan.data_ptr<int>());
   RLB_CUDA_CHECK(cudaGetLastError());
   return plan;
@@ -874,9 +1671,8 @@ at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, a
 
 at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor block_tables,
                               at::Tensor plan, int64_t groups, double scale, double k_scale, double v_scale) {
-  RLB_CHECK(q.is_cuda() && q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.stride(2) == 1 &&
-                q.stride(1) % 2 == 0 && q.stride(0) % 2 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 4 == 0,
-            "shared_prefix_attn: q must be bf16 [rows, heads, dims] with even strides");
+  RLB_CHECK(q.is_cuda() && q.dim() == 3 && q.scalar_type() == at::kBFloat16,
+            "shared_prefix_attn: q must be bf16 [rows, heads, dims]");
   const bool f8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
   RLB_CHECK(f8 || k_cache.scalar_type() == at::kBFloat16, "shared_prefix_attn: the cache must be bf16 or e4m3");
   RLB_CHECK(k_cache.dim() == 4 && k_cache.is_contiguous() && v_cache.is_contiguous() &&
@@ -885,16 +1681,18 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
   const int64_t B = q.size(0), nq = q.size(1), hd = q.size(2), nb = k_cache.size(0), bs = k_cache.size(1),
                 nkv = k_cache.size(2);
   RLB_CHECK(hd == 32 || hd == 64 || hd == 128, "shared_prefix_attn: head_dim must be 32, 64 or 128");
-  RLB_CHECK(k_cache.size(3) == hd && nkv >= 1 && nq >= nkv && nq % nkv == 0 && nq / nkv <= sp::MR,
+  RLB_CHECK(k_cache.size(3) == hd && nkv >= 1 && nq >= nkv && nq % nkv == 0 && nq / nkv <= sp::kMaxHeads,
             "shared_prefix_attn: heads of q and cache do not match");
   RLB_CHECK(nb >= 1 && bs >= 1 && nb * bs < (1LL << 31), "shared_prefix_attn: the cache needs 1 to 2^31 - 1 keys");
   RLB_CHECK(block_tables.is_cuda() && block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt &&
                 block_tables.is_contiguous() && block_tables.size(0) == B && (B == 0 || block_tables.size(1) >= 1),
             "shared_prefix_attn: int32 block tables [rows, pages] expected");
-  const int Gq = nq / nkv, ctas = sp::grid_ctas();
+  const int Gq = nq / nkv;
+  const bool tc = sp::use_tc(hd, bs);
+  const sp::Shape p = sp::shape_of(tc);
   const int units = sp::max_chunks(B, groups, Gq) + B;
   RLB_CHECK(plan.is_cuda() && plan.scalar_type() == at::kInt && plan.is_contiguous() && groups >= 0 &&
-                plan.numel() == sp::plan_ints(ctas, units, B),
+                plan.numel() == sp::plan_ints(p, units, B),
             "shared_prefix_attn: the plan is of another batch");
   for (const at::Tensor& t : {k_cache, v_cache, block_tables, plan})
     RLB_CHECK(t.device() == q.device(), "shared_prefix_attn: all tensors must be on one device");
@@ -903,12 +1701,9 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
   const c10::cuda::CUDAGuard guard(q.device());
   auto out = at::empty({B, nq, hd}, q.options());
   if (B == 0) return out;
-  // keys of a TMA box: a power of two that divides the page, so a box never leaves its page and an
-  // aligned tile is whole boxes.  Below 8 keys (a swizzle period) rows are copied one by one instead.
-  int box = sp::BT;
-  while (bs % box) box /= 2;
-  if (box < 8) box = 0;
-  const long long slots = 2 * B * nq + (long long)ctas * sp::MR;
+  if (q.stride(2) != 1 || q.stride(1) % 8 || q.stride(0) % 8) q = q.contiguous();
+  if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 16) q = q.clone(at::MemoryFormat::Contiguous);
+  const long long slots = 4 * B * nq + 4LL * p.ctas * sp::MR;
   auto part = at::empty({slots * (hd + 2)}, q.options().dtype(at::kFloat));
   sp::Args a;
   a.q = (const sp::bf16*)q.data_ptr();
@@ -920,31 +1715,42 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
   a.table_row = block_tables.size(1);
   a.n_blocks = nb;
   a.block = bs;
-  a.box = box;
+  a.box = sp::box_keys(bs, sp::BT);
   a.plan = plan.data_ptr<int>();
-  a.ctas = ctas;
+  a.ctas = p.ctas;
   a.units = units;
   a.B = B;
   a.nq = nq;
   a.nkv = nkv;
   a.Gq = Gq;
+  a.inv_gq = Gq == 1 ? 0 : (uint32_t)(((1ull << 32) + Gq - 1) / Gq);
   a.scale_log2 = (float)(scale * (f8 ? k_scale : 1.0) * 1.4426950408889634);
   a.part_o = part.data_ptr<float>();
   a.part_ml = a.part_o + slots * hd;
   CUtensorMap tk = {}, tv = {};
-  if (box) {
-    tk = sp::cache_tmap(k_cache, box, f8);
-    tv = sp::cache_tmap(v_cache, box, f8);
+  if (a.box) {
+    tk = sp::cache_tmap(k_cache, a.box, p.tile, f8);
+    tv = sp::cache_tmap(v_cache, a.box, p.tile, f8);
   }
   auto launch = [&](auto hdv, auto f8v) {
     constexpr int HD = decltype(hdv)::value;
     constexpr bool F8 = decltype(f8v)::value;
-    using C = sp::Cfg<HD, F8>;
-    auto kern = sp::shared_prefix_attn_kernel<HD, F8>;
-    RLB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    sp::launch_pdl(kern, ctas, 160, C::SMEM, tk, tv, a);
-    sp::launch_pdl(sp::shared_prefix_combine_kernel<HD>, (int)((B * nq + 3) / 4), 128, 0, (const int*)a.plan, ctas,
-                   units, (int)B, (int)nq, (int)nkv, Gq, (const float*)a.part_o, (const float*)a.part_ml,
+    if constexpr (HD >= 64) {
+      if (tc) {
+        using T = sp::Tc<HD, F8>;
+        auto kern = sp::shared_prefix_tc_kernel<HD, F8>;
+        RLB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM));
+        sp::launch_pdl(kern, p.ctas, T::THREADS, T::SMEM, tk, tv, a);
+      }
+    }
+    if (!tc) {
+      auto kern = sp::shared_prefix_attn_kernel<HD, F8>;
+      constexpr int smem = sp::Gen<HD, F8>::SMEM;
+      RLB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      sp::launch_pdl(kern, p.ctas, 160, smem, tk, tv, a);
+    }
+    sp::launch_pdl(sp::shared_prefix_combine_kernel<HD>, (int)((B * nq + 3) / 4), 128, 0, (const int*)a.plan, p.ctas,
+                   tc ? 2 : 1, units, (int)B, (int)nq, (int)nkv, Gq, (const float*)a.part_o, (const float*)a.part_ml,
                    f8 ? (float)v_scale : 1.f, (sp::bf16*)out.data_ptr());
   };
   auto by_type = [&](auto hdv) {

@@ -235,6 +235,8 @@ class SharedPrefixPlan(NamedTuple):
     groups: int
     heads: int
     kv_heads: int
+    head_dim: int
+    block_size: int
 
 
 def _check_groups(seq_lens, group_starts, prefix_lens):
@@ -247,15 +249,17 @@ def _check_groups(seq_lens, group_starts, prefix_lens):
                          f"starts, got {group_starts.numel()}")
 
 
-def shared_prefix_plan(seq_lens, group_starts, prefix_lens, num_heads: int, num_kv_heads: int) -> SharedPrefixPlan:
+def shared_prefix_plan(seq_lens, group_starts, prefix_lens, num_heads: int, num_kv_heads: int, head_dim: int,
+                       block_size: int) -> SharedPrefixPlan:
     """Plan the attention of one decode step: which CTA takes which keys of which rows.
 
-    The plan depends on the lengths alone (read on the device, without a synchronisation), so one
-    plan serves every layer of the step; lengths that change need a new one.  GPU only."""
+    The plan depends on the lengths and the head and page sizes alone (lengths are read on the
+    device, without a synchronisation), so one plan serves every layer of the step; lengths that
+    change need a new one.  GPU only."""
     _check_groups(seq_lens, group_starts, prefix_lens)
     i32 = [t.to(torch.int32).contiguous() for t in (group_starts, prefix_lens, seq_lens)]
-    buf = ext().shared_prefix_plan(*i32, int(num_heads), int(num_kv_heads))
-    return SharedPrefixPlan(buf, seq_lens.numel(), prefix_lens.numel(), int(num_heads), int(num_kv_heads))
+    key = (int(num_heads), int(num_kv_heads), int(head_dim), int(block_size))
+    return SharedPrefixPlan(ext().shared_prefix_plan(*i32, *key), seq_lens.numel(), prefix_lens.numel(), *key)
 
 
 def shared_prefix_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, group_starts, prefix_lens,
@@ -294,13 +298,11 @@ def shared_prefix_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, 
         if bool(live.any()):  # every row's table is complete: the grouping changes what is read, not the result
             out[live] = paged_decode_attention_ref(q[live], k_cache, v_cache, block_tables[live], seq_lens[live], scale)
         return out
-    nq, nkv = q.shape[1], k_cache.shape[2]
+    key = (q.shape[1], k_cache.shape[2], q.shape[2], k_cache.shape[1])
     if plan is None:
-        plan = shared_prefix_plan(seq_lens, group_starts, prefix_lens, nq, nkv)
-    elif plan[1:] != (B, prefix_lens.numel(), nq, nkv):
-        raise ValueError(f"shared prefix attention: a plan for (rows, groups, heads, KV heads) {plan[1:]} used for "
-                         f"{(B, prefix_lens.numel(), nq, nkv)}")
-    if q.stride(2) != 1 or q.stride(1) % 2 or q.stride(0) % 2 or q.data_ptr() % 4:
-        q = q.contiguous() if not q.is_contiguous() else q.clone()
+        plan = shared_prefix_plan(seq_lens, group_starts, prefix_lens, *key)
+    elif plan[1:] != (B, prefix_lens.numel(), *key):
+        raise ValueError("shared prefix attention: a plan for (rows, groups, heads, KV heads, head dim, block size) "
+                         f"{plan[1:]} used for {(B, prefix_lens.numel(), *key)}")
     return ext().shared_prefix_attn(q, k_cache, v_cache, block_tables.to(torch.int32).contiguous(), plan.buf,
                                     plan.groups, float(scale), float(k_scale), float(v_scale))

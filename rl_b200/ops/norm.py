@@ -116,14 +116,8 @@ def _norm_fp8(x: torch.Tensor, delta, w: torch.Tensor, eps: float, mx: bool):
         q, sc = quant_act_mx(y2) if mx else quant_fp8_group_ref(y2, 128, False)
         return q.view(x.shape), sc, s
 
-    def rows(t):
-        t = t.reshape(-1, H).contiguous()
-        return t if t.data_ptr() % (8 * t.element_size()) == 0 else t.clone()
-
-    wc = w.contiguous()
-    wc = wc if wc.data_ptr() % (8 * wc.element_size()) == 0 else wc.clone()
-    out = ext().rmsnorm_fp8(rows(x), None if delta is None else rows(delta), wc, float(eps), bool(mx), bool(mx))
-    return out[0].view(x.shape), out[1], None if delta is None else out[2].view(x.shape)
+    out = ext().rmsnorm_fp8(x, delta, w, float(eps), bool(mx), bool(mx))
+    return out if delta is not None else (*out, None)
 
 
 def rms_norm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, mx: bool = True):
@@ -135,9 +129,9 @@ def rms_norm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, mx: bool =
     :func:`rl_b200.ops.fp8_gemm.gemm_fp8`.  The hidden size is a multiple of 128 (at most 16384 on a
     GPU).  For inference: an input that needs a gradient is refused.
     """
-    return _norm_fp8(x, None, w, eps, mx)[:2]
+    return tuple(_norm_fp8(x, None, w, eps, mx)[:2])
 
 
 def add_rms_norm_fp8(x: torch.Tensor, delta: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, mx: bool = True):
     """``(q, scales, x + delta)``: :func:`rms_norm_fp8` of the residual sum, which is returned too."""
-    return _norm_fp8(x, delta, w, eps, mx)
+    return tuple(_norm_fp8(x, delta, w, eps, mx))

@@ -220,7 +220,7 @@ def test_shared_prefix_attention_repeats_and_keeps_its_inputs(cuda_device):
     b = Batch(cuda_device, [16, 8], [700, 300], [701 + i for i in range(16)] + [301 + 40 * i for i in range(8)], 32, 8,
               128, 256)
     kc, vc = b.kc.clone(), b.vc.clone()
-    plan = shared_prefix_plan(b.lens, b.starts, b.prefix, 32, 8)
+    plan = shared_prefix_plan(b.lens, b.starts, b.prefix, 32, 8, 128, 256)
     out = b.run()
     for _ in range(3):
         assert torch.equal(b.run(plan=plan), out)  # one plan for every layer, the same bits every time
@@ -231,7 +231,7 @@ def test_shared_prefix_attention_repeats_and_keeps_its_inputs(cuda_device):
 
 def test_shared_prefix_attention_refuses(cuda_device):
     b = Batch(cuda_device, [2], [64], [70, 80], 8, 2, 128, 16)
-    plan = shared_prefix_plan(b.lens, b.starts, b.prefix, 8, 2)
+    plan = shared_prefix_plan(b.lens, b.starts, b.prefix, 8, 2, 128, 16)
     with pytest.raises(ValueError):  # a plan of another batch
         b.run(plan=plan._replace(rows=3))
     with pytest.raises(RuntimeError):
