@@ -15,6 +15,10 @@ Design (B200-first)
   are handed out per sequence up front for ``prompt + max_new_tokens``.
 * Prefill runs all prompts packed (THD) through the varlen attention kernel
   and writes K/V to the cache.
+* Identical prompts (a GRPO group's samples) are prefilled once.  The other rows get
+  their prompt's pages copied, or (``mcore_generation_config.enable_shared_prefix_attention``)
+  forked: block tables share its full pages, only the last, partly filled page is copied,
+  and decode attends to each group's prompt once for all of its rows.
 * Decode runs ENTIRELY on the device: one CUDA graph per batch bucket does
   slot computation, the model step, LM head, sampling, the output write and
   stop-token / length bookkeeping.  The host only replays the graph and reads
@@ -32,6 +36,7 @@ import torch
 from rl_b200.distributed.batched_data_dict import BatchedDataDict
 from rl_b200.models.transformer import KVCache, TransformerLM
 from rl_b200.ops._ext import add_launches, launch_count
+from rl_b200.ops.cache_pages import copy_cache_pages
 from rl_b200.ops.sampling import sample_tokens
 
 __all__ = ["RolloutEngine"]
@@ -57,6 +62,9 @@ class _DecodeState:
         self.seq_lens = torch.zeros(B, dtype=i32, device=device)
         self.slot = torch.zeros(B, dtype=i64, device=device)
         self.block_tables = torch.zeros(B, max_blocks, dtype=i32, device=device)
+        # rows that share a prompt: their bounds and the prompt's length (unused groups are empty)
+        self.group_starts = torch.zeros(B + 1, dtype=i32, device=device)
+        self.prefix_lens = torch.zeros(B, dtype=i32, device=device)
         self.done = torch.ones(B, dtype=torch.bool, device=device)
         self.gen_len = torch.zeros(B, dtype=i32, device=device)
         self.max_new = torch.zeros(B, dtype=i32, device=device)
@@ -118,6 +126,8 @@ class RolloutEngine:
         # generated token's distribution ("sampler_topk_token_ids / _logprobs")
         self.record_sampler_topk = 0
         self._topk_steps: Optional[list] = None
+        # shared prompts of the call in progress, see generate()
+        self._prompts: Optional[tuple] = None
 
     # ------------------------------------------------------------ lifecycle
     def prepare_for_generation(self, num_seqs: Optional[int] = None) -> bool:
@@ -224,7 +234,7 @@ class RolloutEngine:
         dev = self.device
         bs = self.block_size
         nblk = self.max_blocks_per_seq
-        block_tables = (torch.arange(B * nblk, dtype=torch.int32).view(B, nblk) + 1).to(dev)  # block 0 = scratch
+        tables = torch.arange(B * nblk, dtype=torch.int32).view(B, nblk) + 1  # block 0 = scratch
 
         # ---- prefill (packed prompts) ----
         lens_l = lengths.tolist()
@@ -242,6 +252,15 @@ class RolloutEngine:
         chunk_tokens = int(mg.get("max_tokens", 16384)) if (mg.get("enable_chunked_prefill", True)
                                                              and not recording and ep <= 1) else 0
         rep, inv = self._unique_prompts(input_ids, lens_l) if dedup else (list(range(B)), list(range(B)))
+        share = bool(mg.get("enable_shared_prefix_attention", False)) and len(rep) < B
+        if share and dev.type == "cuda" and self.model.hd not in (32, 64, 128):
+            raise ValueError(f"enable_shared_prefix_attention needs a head_dim of 32, 64 or 128, not {self.model.hd}")
+        if share:
+            for b, u in enumerate(inv):  # forked rows read their prompt's full pages where it was prefilled
+                tables[b, : lens_l[b] // bs] = tables[rep[u], : lens_l[b] // bs]
+        block_tables = tables.to(dev)
+        # (prompt of every row, prompt lengths) while decode shares prompts
+        self._prompts = (torch.tensor(inv), torch.tensor([lens_l[r] for r in rep])) if share else None
         if recording:
             self.model.router_record = {}
         h_parts = []
@@ -250,7 +269,7 @@ class RolloutEngine:
             h_parts.append(self._prefill_rows(input_ids, rows, lens_l, block_tables, spec))
         h = torch.cat(h_parts) if len(h_parts) > 1 else h_parts[0]
         if len(rep) < B:
-            self._copy_prompt_blocks(rep, inv, lens_l, block_tables, spec)
+            self._copy_prompt_blocks(rep, inv, lens_l, tables, spec)
             h = h[torch.tensor(inv, device=h.device)]
         if self._eagle_fprev_rows:
             self._eagle_fprev = torch.stack([self._eagle_fprev_rows[rep[u]] for u in inv])
@@ -380,29 +399,37 @@ class RolloutEngine:
             self.draft.forward_prefill(flat, positions, cu_d, max(rl), self.draft_kv, slot, last_idx)
         return h
 
-    def _copy_prompt_blocks(self, rep: list[int], inv: list[int], lens: list, block_tables: torch.Tensor,
+    def _copy_prompt_blocks(self, rep: list[int], inv: list[int], lens: list, tables: torch.Tensor,
                             spec: bool) -> None:
-        """Give every duplicate row the KV blocks of its prompt's prefilled row."""
+        """Give every duplicate row the KV of its prompt's prefilled row in the pages of its own
+        (``tables`` on the host): all of them, or the last one where the full pages are shared."""
         bs = self.block_size
-        src, dst = [], []
+        rows = tables.tolist()
+        src, dst, tokens = [], [], []
         for b, u in enumerate(inv):
-            r = rep[u]
-            if r == b:
-                continue
-            nb = -(-lens[b] // bs)
-            src.append(block_tables[r, :nb])
-            dst.append(block_tables[b, :nb])
-        if not src:
-            return
-        src_t, dst_t = torch.cat(src).long(), torch.cat(dst).long()
+            for j in range(-(-lens[b] // bs)):
+                if rows[b][j] != rows[rep[u]][j]:
+                    src.append(rows[rep[u]][j])
+                    dst.append(rows[b][j])
+                    tokens.append(min(bs, lens[b] - j * bs))
         for cache in ([self.kv, self.draft_kv] if spec else [self.kv]):
-            st = cache.storage
-            if st.element_size() == 1:
-                st = st.view(torch.uint8)  # fp8 caches: copy the bytes
-            for layer in range(st.shape[0]):  # per layer: the gathered blocks stay small
-                for kv in range(2):
-                    t = st[layer, kv]
-                    t.index_copy_(0, dst_t, t.index_select(0, src_t))
+            copy_cache_pages(cache.storage, src, dst, tokens)
+
+    def _prefix_groups(self, rows: Optional[torch.Tensor] = None, width: int = 1, out=None):
+        """Bounds and prompt lengths of the runs of ``rows`` (default: all) that share a prompt,
+        ``width`` batch rows each; written to ``out`` = (starts, lengths), whose unused groups are empty."""
+        prompt, lens = self._prompts
+        p = prompt if rows is None else prompt[rows.cpu()]
+        ids, counts = torch.unique_consecutive(p, return_counts=True)
+        starts = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]) * width
+        if out is None:
+            return starts.to(self.device, torch.int32), lens[ids].to(self.device, torch.int32)
+        n = len(ids)
+        out[0].fill_(int(starts[-1]))
+        out[0][: n + 1] = starts.to(out[0])
+        out[1].zero_()
+        out[1][:n] = lens[ids].to(out[1])
+        return out
 
     @staticmethod
     def _sampler_topk(logits: torch.Tensor, temperature: float, k: int):
@@ -466,6 +493,8 @@ class RolloutEngine:
         pos0 = lengths.to(torch.int64).clone()       # position of `last`
         ar = torch.arange(k + 1, device=dev)
         bt_rows = block_tables.repeat_interleave(k + 1, 0)
+        prefix = self._prefix_groups() if self._prompts is not None else None
+        prefix_rows = self._prefix_groups(width=k + 1) if self._prompts is not None else None
         temp = temperature if temperature > 0 else 0.0
         rnd = 0
         kind = getattr(self, "draft_kind", "lm")
@@ -493,7 +522,8 @@ class RolloutEngine:
                                         maxlen)
                     h = f
                 else:
-                    h = self.draft.forward_decode(x, p, self.draft_kv, block_tables, p + 1, slot, maxlen)
+                    h = self.draft.forward_decode(x, p, self.draft_kv, block_tables, p + 1, slot, maxlen,
+                                                  prefix=prefix)
                 lg = self.draft.logits_infer(h)
                 x, _ = sample_tokens(lg, temp if temp > 0 else 1.0, 1 if temp == 0 else None, 1.0, seed=self.seed + 17,
                                      offset=(self.calls << 24) + rnd * (k + 1) + j)
@@ -507,7 +537,8 @@ class RolloutEngine:
             if eagle:
                 self.model.capture_layers, self.model.captured = self.draft.aux_layers, None
             try:
-                h = self.model.forward_decode(rows_tok, rows_pos, self.kv, bt_rows, rows_pos + 1, slot, maxlen)
+                h = self.model.forward_decode(rows_tok, rows_pos, self.kv, bt_rows, rows_pos + 1, slot, maxlen,
+                                              prefix=prefix_rows)
                 vfeats = (torch.cat([self.model.captured[i] for i in self.draft.aux_layers], -1).view(B, k + 1, -1)
                           if eagle else None)
             finally:
@@ -590,7 +621,7 @@ class RolloutEngine:
         while rows.numel() > 0 and step_done < max_new:
             nb = next(b for b in _buckets(self.max_num_seqs) if b >= rows.numel()) \
                 if rows.numel() <= self.max_num_seqs else rows.numel()
-            st = self._state(nb, max_new, (temperature, top_k, top_p))
+            st = self._state(nb, max_new, (temperature, top_k, top_p, self._prompts is not None))
             n = rows.numel()
             st.stop.fill_(-1)
             st.stop[: min(len(stop_ids), st.stop.numel())] = stop[: st.stop.numel()] if stop_ids else -1
@@ -602,6 +633,8 @@ class RolloutEngine:
             st.positions[:n] = (lengths[rows] + step_done - 1).to(torch.int32)
             st.block_tables.zero_()
             st.block_tables[:n] = block_tables[rows]
+            if self._prompts is not None:
+                self._prefix_groups(rows, out=(st.group_starts, st.prefix_lens))
             st.gen_len.zero_()
             st.gen_len[:n] = glen[rows]
             st.max_new.fill_(max_new)
@@ -656,7 +689,8 @@ class RolloutEngine:
         st.slot.copy_(blk.long() * bs + (st.positions % bs).long())
         st.seq_lens.copy_(st.positions + 1)
         h = self.model.forward_decode(st.tokens, st.positions, self.kv, st.block_tables, st.seq_lens, st.slot,
-                                      self.max_model_len)
+                                      self.max_model_len,
+                                      prefix=(st.group_starts, st.prefix_lens) if self._prompts is not None else None)
         logits = self.model.logits_infer(h)
         from rl_b200.ops.sampling import sample_tokens_graphable
 
@@ -704,13 +738,14 @@ class RolloutEngine:
         bs = self.block_size
         tokens = tok0.clone()
         positions = lengths.to(torch.int32).clone()
+        prefix = self._prefix_groups() if self._prompts is not None else None
         for step in range(1, max_new):
             if bool(done.all()):
                 break
             blk = block_tables.gather(1, (positions // bs).long().unsqueeze(1)).squeeze(1)
             slot = blk.long() * bs + (positions % bs).long()
             h = self.model.forward_decode(tokens, positions, self.kv, block_tables, positions + 1, slot,
-                                          self.max_model_len)
+                                          self.max_model_len, prefix=prefix)
             if self._route_steps is not None:
                 self._route_steps.append(self._take_routes())
             logits = self.model.logits_infer(h)

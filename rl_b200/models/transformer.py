@@ -38,7 +38,8 @@ import torch.utils.checkpoint as ckpt
 
 from rl_b200.models.config import ModelConfig
 from rl_b200.ops.activation import swiglu
-from rl_b200.ops.attention import flash_attn_varlen, flash_attn_varlen_fwd, paged_decode_attention, write_kv_cache
+from rl_b200.ops.attention import (flash_attn_varlen, flash_attn_varlen_fwd, paged_decode_attention,
+                                   shared_prefix_decode_attention, shared_prefix_plan, write_kv_cache)
 from rl_b200.ops.linear import linear
 from rl_b200.ops.norm import add_rms_norm, rms_norm
 from rl_b200.ops.rope import apply_rope_qkv, build_rope_cache
@@ -971,22 +972,36 @@ class TransformerLM(nn.Module):
 
     @torch.no_grad()
     def forward_decode(self, tokens, positions, kv: KVCache, block_tables, seq_lens, slot_mapping,
-                       max_seq_len: int = 0, hidden_in: Optional[torch.Tensor] = None) -> torch.Tensor:
+                       max_seq_len: int = 0, hidden_in: Optional[torch.Tensor] = None,
+                       prefix: Optional[tuple] = None) -> torch.Tensor:
         """One decode step for ``B`` sequences: ``tokens [B]`` -> hidden ``[B, H]``
-        (``hidden_in`` replaces the token embeddings)."""
+        (``hidden_in`` replaces the token embeddings; ``prefix`` = (group starts, prefix
+        lengths) of rows that share their first keys, see ``shared_prefix_decode_attention``)."""
         self._in_rollout = True
         try:
             return self._forward_decode(tokens, positions, kv, block_tables, seq_lens, slot_mapping, max_seq_len,
-                                        hidden_in)
+                                        hidden_in, prefix)
         finally:
             self._in_rollout = False
 
+    def _decode_attention(self, kv: KVCache, block_tables, seq_lens, max_seq_len, prefix):
+        """The decode attention of one step as ``attend(q, layer)``; with a shared prefix the step is
+        planned here, once for all layers."""
+        if prefix is None:
+            return lambda q, i: paged_decode_attention(q, *kv.layer(i), block_tables, seq_lens,
+                                                       max_seq_len=max_seq_len, k_scale=kv.scales(i)[0],
+                                                       v_scale=kv.scales(i)[1])
+        plan = (shared_prefix_plan(seq_lens, *prefix, self.nq, self.nkv, self.hd, kv.block_size)
+                if seq_lens.is_cuda else None)
+        return lambda q, i: shared_prefix_decode_attention(q, *kv.layer(i), block_tables, seq_lens, *prefix,
+                                                           k_scale=kv.scales(i)[0], v_scale=kv.scales(i)[1], plan=plan)
+
     def _forward_decode(self, tokens, positions, kv, block_tables, seq_lens, slot_mapping, max_seq_len,
-                        hidden_in=None):
+                        hidden_in=None, prefix=None):
         ar = self._decode_ar_op(tokens.shape[0]) if not self.cfg.is_moe else None
+        attend = self._decode_attention(kv, block_tables, seq_lens, max_seq_len, prefix)
         if ar is not None:
-            return self._forward_decode_fused_ar(tokens, positions, kv, block_tables, seq_lens, slot_mapping,
-                                                 max_seq_len, ar, hidden_in)
+            return self._forward_decode_fused_ar(tokens, positions, kv, slot_mapping, attend, ar, hidden_in)
         x = self.embed_full(tokens) if hidden_in is None else hidden_in
         resid = None
         eps = self.cfg.rms_eps
@@ -997,10 +1012,8 @@ class TransformerLM(nn.Module):
             qkv = self._qkv(i, None, positions, qkv)
             q, k, v = self._split_heads(qkv)
             kc, vc = kv.layer(i)
-            ks, vs = kv.scales(i)
-            write_kv_cache(k, v, kc, vc, slot_mapping, ks, vs)
-            o = paged_decode_attention(q, kc, vc, block_tables, seq_lens, max_seq_len=max_seq_len,
-                                       k_scale=ks, v_scale=vs)
+            write_kv_cache(k, v, kc, vc, slot_mapping, *kv.scales(i))
+            o = attend(q, i)
             a = self._tp_sum(self._lin_infer(o.reshape(o.shape[0], -1), p + "self_attn.o_proj.weight"))
             m, s2 = self._norm_mlp_infer(i, s, a)
             x, resid = s2, m
@@ -1008,8 +1021,7 @@ class TransformerLM(nn.Module):
         h, _ = add_rms_norm(x, resid, self._params["model.norm.weight"], eps)
         return h
 
-    def _forward_decode_fused_ar(self, tokens, positions, kv, block_tables, seq_lens, slot_mapping, max_seq_len, ar,
-                                 hidden_in=None):
+    def _forward_decode_fused_ar(self, tokens, positions, kv, slot_mapping, attend, ar, hidden_in=None):
         """Decode step with every row-parallel output reduced by the fused
         peer-memory all-reduce + residual add + RMSNorm (no NCCL in the step)."""
         eps = self.cfg.rms_eps
@@ -1021,10 +1033,8 @@ class TransformerLM(nn.Module):
             qkv = self._qkv(i, h, positions)
             q, k, v = self._split_heads(qkv)
             kc, vc = kv.layer(i)
-            ks, vs = kv.scales(i)
-            write_kv_cache(k, v, kc, vc, slot_mapping, ks, vs)
-            o = paged_decode_attention(q, kc, vc, block_tables, seq_lens, max_seq_len=max_seq_len,
-                                       k_scale=ks, v_scale=vs)
+            write_kv_cache(k, v, kc, vc, slot_mapping, *kv.scales(i))
+            o = attend(q, i)
             a = self._lin_infer(o.reshape(o.shape[0], -1), p + "self_attn.o_proj.weight")
             h2 = ar(a, s, self._params[p + "post_attention_layernorm.weight"], eps)
             gu = self._lin_infer(h2, p + "mlp.gate_up_proj.weight")

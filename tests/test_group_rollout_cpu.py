@@ -122,3 +122,52 @@ def test_norm_fp8_refuses():
         rms_norm_fp8(x.requires_grad_(True), w)
     with torch.no_grad():
         rms_norm_fp8(x, w)
+
+
+# ------------------------------------------------------------------------ rollout engine
+def _worker(mg: dict):
+    from rl_b200.models.config import get_model_config
+    from rl_b200.models.policy.worker import PolicyWorker
+    from rl_b200.parallel.state import single_process_state
+
+    pcfg = {"max_total_sequence_length": 96, "precision": "float32", "train_global_batch_size": 12,
+            "generation": {"temperature": 1.0, "max_new_tokens": 12,
+                           "mcore_generation_config": {"block_size_tokens": 16, **mg}}}
+    return PolicyWorker(pcfg, model_cfg=get_model_config("tiny-llama"),
+                        pstate=single_process_state(torch.device("cpu")), seed=3)
+
+
+def _batch(order=None):
+    from rl_b200.distributed.batched_data_dict import BatchedDataDict
+
+    g = torch.Generator().manual_seed(0)
+    lens = torch.tensor([5, 32, 40, 17]).repeat_interleave(3)
+    ids = torch.randint(0, 512, (4, 40), generator=g).repeat_interleave(3, 0)
+    order = torch.arange(12) if order is None else order
+    return BatchedDataDict({"input_ids": ids[order], "input_lengths": lens[order]})
+
+
+@pytest.mark.parametrize("order", [None, [0, 3, 1, 6, 7, 4, 5, 8, 9, 2, 11, 10]])
+def test_shared_prompt_rollout_equals_copied_prompts(order):
+    data = _batch(None if order is None else torch.tensor(order))
+    ref = _worker({}).generate(data, greedy=True)
+    w = _worker({"enable_shared_prefix_attention": True})
+    out = w.generate(data, greedy=True)
+    assert torch.equal(out["output_ids"], ref["output_ids"])
+    torch.testing.assert_close(out["logprobs"], ref["logprobs"], atol=1e-5, rtol=0)
+    assert w.engine._prompts is not None
+    starts, lens = w.engine._prefix_groups()
+    if order is None:
+        assert starts.tolist() == [0, 3, 6, 9, 12] and lens.tolist() == [5, 32, 40, 17]
+    assert w.engine._prefix_groups(width=3)[0].tolist() == [3 * s for s in starts.tolist()]
+    out_starts, out_lens = torch.full((14,), 77, dtype=torch.int32), torch.full((13,), 77, dtype=torch.int32)
+    w.engine._prefix_groups(torch.tensor([0, 1, 5, 11]), out=(out_starts, out_lens))
+    assert out_starts[-1] == 4 and out_lens[-1] == 0 and (out_starts.diff() >= 0).all()
+
+
+def test_rollout_without_duplicates_does_not_share():
+    w = _worker({"enable_shared_prefix_attention": True})
+    data = _batch(torch.tensor([0, 3, 6, 9]))
+    ref = _worker({}).generate(data, greedy=True)
+    assert torch.equal(w.generate(data, greedy=True)["output_ids"], ref["output_ids"])
+    assert w.engine._prompts is None

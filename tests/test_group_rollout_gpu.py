@@ -481,3 +481,68 @@ def test_norm_fp8_special_values_views_and_empty(cuda_device):
         rms_norm_fp8(torch.zeros(2, 16512, device=cuda_device), torch.ones(16512, device=cuda_device))
     with pytest.raises(ValueError):
         rms_norm_fp8(x, w.cpu())
+
+
+# -------------------------------------------------------------------- the three together
+def test_forked_pages_attend_like_copied_ones(cuda_device):
+    # a prompt of 150 tokens in row 0's pages: forked (full pages shared, the last one copied) and copied whole
+    b = Batch(cuda_device, [4], [150], [151, 180, 150, 200], 8, 2, 128, 16, share=False)
+    want = b.run()
+    b.check(want)
+    storage = torch.stack([b.kc, b.vc])[None]  # [layers, 2, pages, block, heads, dims]
+    own = b.tables.cpu()
+    for forked in (True, False):
+        cache, tables = storage.clone(), own.clone()
+        first = 150 // 16 if forked else 0
+        for r in range(1, 4):
+            cache[0, :, own[r, :9].long()] = float("nan")  # the prompt's pages of the row, but the partly filled one's rest
+            cache[0, :, own[r, 9].long(), :6] = float("nan")
+            tables[r, :first] = own[0, :first]
+        pairs = [(int(own[0, j]), int(own[r, j]), min(16, 150 - 16 * j)) for r in range(1, 4) for j in range(first, 10)]
+        copy_cache_pages(cache, *zip(*pairs))
+        b.kc, b.vc, b.tables = cache[0, 0], cache[0, 1], tables.to(cuda_device)
+        assert torch.equal(b.run(), want)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("graphs", [False, True])
+def test_shared_prompt_rollout(cuda_device, graphs, fp8):
+    """Prefill once, fork, decode with the shared prompt (and, fp8, with norms that quantise): the
+    sampler's log-probs are the trainer's, within what rollouts with copied prompts are held to."""
+    from rl_b200.distributed.batched_data_dict import BatchedDataDict
+    from rl_b200.models.config import ModelConfig
+    from rl_b200.models.policy.worker import PolicyWorker
+
+    cfg = ModelConfig(name="small", vocab_size=2048, hidden_size=512, num_layers=3, num_heads=8, num_kv_heads=2,
+                      head_dim=64, ffn_hidden_size=1408, rope_theta=10000.0, max_position_embeddings=1024)
+    pcfg = {"model_name": "small", "max_total_sequence_length": 320, "precision": "bfloat16",
+            "train_global_batch_size": 16, "train_micro_batch_size": 4,
+            "generation": {"temperature": 1.0, "top_p": 1.0, "top_k": None, "max_new_tokens": 40,
+                           "mcore_generation_config": {"block_size_tokens": 16,
+                                                       "enable_shared_prefix_attention": True}},
+            "sequence_packing": {"train_mb_tokens": 2048, "logprob_mb_tokens": 2048}}
+    if fp8:
+        pcfg["generation"]["vllm_cfg"] = {"precision": "fp8", "pow2_weight_scaling_factors": True,
+                                          "pow2_activation_scaling_factors": True}
+    w = PolicyWorker(pcfg, model_cfg=cfg, seed=0)
+    w.engine.use_cuda_graphs = graphs
+    w.engine.sync_every = 8
+    g = torch.Generator().manual_seed(1)
+    lens = torch.tensor([200, 33, 64, 257]).repeat_interleave(4)
+    ids = torch.randint(0, 2048, (4, 257), generator=g).repeat_interleave(4, 0)
+    data = BatchedDataDict({"input_ids": ids, "input_lengths": lens})
+    try:
+        for _ in range(2):  # the second call replays the first one's graphs
+            out = w.generate(data)
+            batch = BatchedDataDict({"input_ids": out["output_ids"],
+                                     "input_lengths": out["unpadded_sequence_lengths"]})
+            lp = w.get_logprobs(batch)["logprobs"]
+            mask = torch.zeros_like(lp, dtype=torch.bool)
+            for i in range(16):
+                mask[i, int(lens[i]): int(out["unpadded_sequence_lengths"][i])] = True
+            diff = (lp - out["logprobs"])[mask].abs()
+            assert mask.sum() > 16 and float(diff.mean()) < (0.1 if fp8 else 0.02)
+            _ext.check_device_errors()
+    finally:
+        w.shutdown()
+    assert w.engine.stats_last_prefill["prefilled"] == 4
