@@ -424,30 +424,45 @@ struct Feed {
     if (!s.done()) seek(a, tile);
     else begin(a, tile, line + 1);
   }
-  // bytes of a load of up to C::KEYS keys
-  template <typename C>
-  __device__ __forceinline__ uint32_t bytes(int box) const {
-    return (uint32_t)((min(C::KEYS, s.k1 - key) + box - 1) / box * box * C::RB);
-  }
-  // the next KEYS keys (whole boxes, none behind the last key) of one cache
-  template <typename C>
-  __device__ __forceinline__ void load(const Args& a, const CUtensorMap* tm, int box, uint32_t dst, uint32_t bar) {
-    for (int r = 0; r < C::KEYS && key < s.k1; r += box) {
-      if (elect_one()) {  // a box that is the whole stage brings all spans of its keys, a smaller one goes span by span
-        tma_4d(dst + r * C::BOXB, tm, bar, s.kvh, z, 0);
-        if (C::NBOX > 1 && box < C::KEYS) tma_4d(dst + C::KEYS * C::BOXB + r * C::BOXB, tm, bar, s.kvh, z, 1);
-      }
-      __syncwarp();
-      key += box;
+  // the next C::KEYS keys of one cache (whole boxes, none behind the last key).  All copies are issued by one
+  // straight piece of code: entering it costs ten times what a further copy in it does.
+  template <typename C, int BOX>
+  __device__ __forceinline__ void load_boxes(const Args& a, const CUtensorMap* tm, uint32_t dst, uint32_t bar) {
+    constexpr int NB = C::KEYS / BOX;
+    int at[NB], n = 0;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      at[b] = z;
       if (key < s.k1) {
-        off += box;
-        z += box;
-        if (off == a.block) {
-          off = 0;
-          z = pages.get(a, s.trow, ++p) * a.block;
+        ++n;
+        key += BOX;
+        if (key < s.k1) {
+          off += BOX;
+          z += BOX;
+          if (off == a.block) {
+            off = 0;
+            z = pages.get(a, s.trow, ++p) * a.block;
+          }
         }
       }
     }
+    if (elect_one()) {
+      mbar_expect_tx(bar, n * BOX * C::RB);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        if (b < n) {
+          tma_4d(dst + b * BOX * C::BOXB, tm, bar, s.kvh, at[b], 0);
+          if (C::NBOX > 1) tma_4d(dst + (C::KEYS + b * BOX) * C::BOXB, tm, bar, s.kvh, at[b], 1);
+        }
+    }
+    __syncwarp();
+  }
+  template <typename C>
+  __device__ __forceinline__ void load(const Args& a, const CUtensorMap* tm, uint32_t dst, uint32_t bar) {
+    if (a.box == 64) load_boxes<C, 64>(a, tm, dst, bar);
+    else if (a.box == 32) load_boxes<C, 32>(a, tm, dst, bar);
+    else if (a.box == 16) load_boxes<C, 16>(a, tm, dst, bar);
+    else load_boxes<C, 8>(a, tm, dst, bar);
   }
 };
 
@@ -738,7 +753,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      mbar_init(bar_full + 8 * s, a.box ? 1 : 32);
+      mbar_init(bar_full + 8 * s, a.box ? 2 : 32);  // K and V, or every lane of the producer
       mbar_init(bar_empty + 8 * s, 4);
     }
     *abort_flag = 0;
@@ -755,11 +770,9 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
       if (!mbar_wait_err(bar_empty + 8 * st, ((k / ST) & 1) ^ 1, abort_flag, &g_shared_prefix_error, kErrWait)) break;
       const uint32_t sk = base + st * 2 * C::BYTES, sv = sk + C::BYTES;
       if (a.box) {
-        if (elect_one()) mbar_expect_tx(bar_full + 8 * st, 2 * f.template bytes<C>(a.box));
-        __syncwarp();
         Feed v = f;
-        v.template load<C>(a, &tv, a.box, sv, bar_full + 8 * st);
-        f.template load<C>(a, &tk, a.box, sk, bar_full + 8 * st);
+        v.template load<C>(a, &tv, sv, bar_full + 8 * st);
+        f.template load<C>(a, &tk, sk, bar_full + 8 * st);
       } else {
         const int key = f.s.k0 + f.s.j * BT;
         for (int r = 0; r < BT; ++r) {
@@ -869,12 +882,12 @@ struct Tc {
   // K tiles behind it.
   static constexpr int KN = F8 ? (HD == 128 ? 1 : 2) : (HD == 128 ? 2 : 4);
   static constexpr int VN = F8 ? (HD == 128 ? 2 : 3) : (HD == 128 ? 3 : 6);
-  static constexpr int RN = F8 ? (HD == 128 ? 4 : 8) : 0;
+  static constexpr int RN = F8 ? (HD == 128 ? 2 : 4) : 0;  // of each
   static constexpr int QB = 5;                     // query buffers: one for the prefix line, up to 4 for the suffix line
-  static constexpr int BARS = 2 * (KN + VN + RN) + 2 * QB + 4 + 4;
-  static constexpr int STAT = 2 * MR * 8 + (4 + 2 + 1 + 1) * MR * 4;  // of a softmax group, see Stat
+  static constexpr int BARS = 2 * (KN + VN + 2 * RN) + 2 * QB + 4 + 4;
+  static constexpr int STAT = (2 + 4 + 2 + 1 + 1) * MR * 4;  // of a softmax group, see Stat
   static constexpr int SMEM =
-      1024 + Q + 2 * P + (KN + VN) * E::BYTES + RN * R::BYTES + 2 * STAT + (MR + 16) * 4 + BARS * 8 + 16;
+      1024 + Q + 2 * P + (KN + VN) * E::BYTES + 2 * RN * R::BYTES + 2 * STAT + (MR + 16) * 4 + BARS * 8 + 16;
   static constexpr uint32_t COLS = 512;  // tensor memory: S four times 64, O twice 64
   static constexpr uint32_t FMT = (1u << 4) | (8u << 24) | (F8 ? 0u : (1u << 7) | (1u << 10));  // M 128, f16 or bf16
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -1001,7 +1014,7 @@ constexpr float kNoMax = -1e30f;  // where a row has no score yet: every score e
 
 // what the threads of a softmax group share
 struct Stat {
-  long long* slot;  // [2][MR] where the partials go, of a segment and of the one before
+  int* slot;        // [2][MR] where the partials go, of a segment and of the one before
   float* red;       // [4][MR] per warp: maxima, sums
   float* m;         // [2][MR] reference scores in use (log2)
   float* alpha;     // [MR]
@@ -1045,31 +1058,12 @@ struct Softmax {
     return live ? top : 0.f;
   }
 
-  // the scores of the tile's first key, which is always one of the row's (thread 0)
-  static __device__ __forceinline__ void refer(uint32_t t_s, float scale, float* sm, const float* sc) {
-#pragma unroll
-    for (int h = 0; h < N; h += 16) {
-      float y[16];
-      tmem_load<16>(t_s + h, y);
-      if ((threadIdx.x & 31) == 0)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = y[i] * (F8 ? sc[h + i] : scale);
-          sm[h + i] = x == -INFINITY ? kNoMax : x;
-        }
-    }
-  }
-
   // one tile up to P (packed in p) and the sums of the rounded P in l; wait_o() waits for the group's
   // product before
   template <typename W>
   static __device__ __forceinline__ void tile(int wg, uint32_t t_s, uint32_t t_o, bool live, bool first, float scale,
                                               const Stat& st, float* sm, float* l, uint32_t* p, int r, W wait_o) {
     const int warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-    if (first) {
-      if (warp4 == 0) refer(t_s, scale, sm, st.c);
-      group_sync(wg);
-    }
     if (group_any(wg, weights(p, t_s, live, scale, sm, st.c) > kMost)) {
 #pragma unroll
       for (int h = 0; h < N; h += H) {
@@ -1153,16 +1147,30 @@ struct Softmax {
 
 };
 
+// the scores of a segment's first key (of the group), by the warp that has it
+template <bool F8>
+__device__ __forceinline__ void refer(uint32_t t_s, int cols, float scale, float* sm, const float* sc) {
+  for (int h = 0; h < cols; h += 16) {
+    float y[16];
+    tmem_load<16>(t_s + h, y);
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = y[i] * (F8 ? sc[h + i] : scale);
+        sm[h + i] = x == -INFINITY ? kNoMax : x;
+      }
+  }
+}
 // a segment's outputs: thread r has dim r
 template <int HD>
-__device__ __forceinline__ void store_o(uint32_t t_o, const long long* slot, float* part_o, int rn, int r) {
+__device__ __forceinline__ void store_o(uint32_t t_o, const int* slot, float* part_o, int rn, int r) {
   for (int h = 0; h < rn; h += 16) {
     float o[16];
     tmem_load<16>(t_o + h, o);
     if (r < HD)
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (h + i < rn) part_o[slot[h + i] * HD + r] = o[i];
+        if (h + i < rn) part_o[(long long)slot[h + i] * HD + r] = o[i];
   }
 }
 
@@ -1181,17 +1189,17 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
   const uint32_t s_p = s_q + T::Q;                     // [2] P of the softmax groups
   const uint32_t s_k = s_p + 2 * T::P;                 // [KN]
   const uint32_t s_v = s_k + T::KN * E::BYTES;         // [VN]
-  const uint32_t s_r = s_v + T::VN * E::BYTES;         // [RN]
-  uint8_t* g_stat = gbase + (s_r - base) + T::RN * R::BYTES;
+  const uint32_t s_r = s_v + T::VN * E::BYTES;         // [2][RN] raw K, raw V
+  uint8_t* g_stat = gbase + (s_r - base) + 2 * T::RN * R::BYTES;
   float* q_factor = reinterpret_cast<float*>(g_stat + 2 * T::STAT);  // of the rows of the query buffer
   uint64_t* bars = reinterpret_cast<uint64_t*>(q_factor + MR + 16);
   const uint32_t bar_k = smem_u32(bars);               // [KN] K ready for the products
   const uint32_t bar_kfree = bar_k + 8 * T::KN;        // [KN] K read
   const uint32_t bar_v = bar_kfree + 8 * T::KN;        // [VN] V ready
   const uint32_t bar_vfree = bar_v + 8 * T::VN;        // [VN] V read
-  const uint32_t bar_r = bar_vfree + 8 * T::VN;        // [RN] raw tile landed
-  const uint32_t bar_rfree = bar_r + 8 * T::RN;        // [RN] raw tile converted
-  const uint32_t bar_q = bar_rfree + 8 * T::RN;        // [QB] query rows ready
+  const uint32_t bar_r = bar_vfree + 8 * T::VN;        // [2][RN] raw tile landed
+  const uint32_t bar_rfree = bar_r + 16 * T::RN;       // [2][RN] raw tile converted
+  const uint32_t bar_q = bar_rfree + 16 * T::RN;       // [QB] query rows ready
   const uint32_t bar_qfree = bar_q + 8 * T::QB;        // [QB] query rows (and factors) read
   const uint32_t bar_s = bar_qfree + 8 * T::QB;        // [4] S complete
   const uint32_t bar_p = bar_s + 32;                   // [2] S read, P written, O rescaled
@@ -1212,12 +1220,12 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
       mbar_init(bar_v + 8 * i, F8 ? 4 : 1);
       mbar_init(bar_vfree + 8 * i, 1);
     }
-    for (int i = 0; i < T::RN; ++i) {
+    for (int i = 0; i < 2 * T::RN; ++i) {
       mbar_init(bar_r + 8 * i, 1);
       mbar_init(bar_rfree + 8 * i, 4);
     }
     for (int i = 0; i < T::QB; ++i) {
-      mbar_init(bar_q + 8 * i, 2);
+      mbar_init(bar_q + 8 * i, 1);
       mbar_init(bar_qfree + 8 * i, F8 ? 3 : 1);
     }
     for (int i = 0; i < 4; ++i) {
@@ -1240,44 +1248,26 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
   tc_fence_after();
   const uint32_t tmem = *tmem_slot, t_o = tmem + 4 * MR;
   pdl_wait();
-  // the walk is the same in every role: tile k belongs to softmax group k & 1.  Tiles are loaded in the order
-  // K_0, K_1, V_0, K_2, V_1, ...
+  // the walk is the same in every role: tile k belongs to softmax group k & 1
   // (e4m3) 512 threads start with 128 registers each; the softmax groups take over what the others do not
   // need: 2 x 80 + 2 x 168 = 496 of 4 x 128
   if (warp < 4) {
   if constexpr (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
-  if (warp == 0) {
-    Feed fk, fv;
-    int nk = 0, nv = 0;
-    auto put = [&](auto is_v) {  // the next K or V tile to its place
-      constexpr int kv = decltype(is_v)::value, n = F8 ? T::RN : kv ? T::VN : T::KN;
-      Feed& d = kv ? fv : fk;
-      const int i = F8 ? nk + nv : kv ? nv : nk, at = i % n;
-      const uint32_t full = (F8 ? bar_r : kv ? bar_v : bar_k) + 8 * at;
-      const uint32_t free = (F8 ? bar_rfree : kv ? bar_vfree : bar_kfree) + 8 * at;
-      const uint32_t dst = (F8 ? s_r : kv ? s_v : s_k) + at * R::BYTES;
-      if (!wait(free, ((i / n) & 1) ^ 1)) return false;
-      if (elect_one()) mbar_expect_tx(full, d.template bytes<R>(a.box));
-      __syncwarp();
-      d.template load<R>(a, kv ? &tv : &tk, a.box, dst, full);
-      ++(kv ? nv : nk);
-      d.next(a, 128);
-      return true;
-    };
-    const std::integral_constant<int, 0> k_tile;
-    const std::integral_constant<int, 1> v_tile;
-    fk.begin(a, 128);
-    fv.begin(a, 128);
-    bool ok = !fk.valid || put(k_tile);
-    while (ok && fv.valid) ok = (!fk.valid || put(k_tile)) && put(v_tile);
-    if (__any_sync(0xffffffffu, *abort_flag)) {
-      if constexpr (F8) {
-        drain(bar_r, T::RN, nk + nv);
-      } else {
-        drain(bar_k, T::KN, nk);
-        drain(bar_v, T::VN, nv);
-      }
+  if (warp == 0 || warp == 3) {  // K tiles, V tiles
+    const bool v = warp == 3;
+    const int n = F8 ? T::RN : v ? T::VN : T::KN;
+    const uint32_t full = F8 ? bar_r + 8 * v * T::RN : v ? bar_v : bar_k;
+    const uint32_t free = F8 ? bar_rfree + 8 * v * T::RN : v ? bar_vfree : bar_kfree;
+    const uint32_t dst = F8 ? s_r + v * T::RN * R::BYTES : v ? s_v : s_k;
+    Feed f;
+    int k = 0, i = 0;
+    uint32_t parity = 1;
+    for (f.begin(a, 128); f.valid && wait(free + 8 * i, parity); ++k) {
+      f.template load<R>(a, v ? &tv : &tk, dst + i * R::BYTES, full + 8 * i);
+      f.next(a, 128);
+      if (++i == n) i = 0, parity ^= 1;
     }
+    if (__any_sync(0xffffffffu, *abort_flag)) drain(full, n, k);
   } else if (warp == 1) {
     Walk w;
     w.begin(a);
@@ -1336,9 +1326,9 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
       if (w.valid) ok = issue_s();
     }
   } else {
-    // query rows, half of them a warp: LPR lanes a row, 16 bytes each; rows up to the segment's columns are zero
-    constexpr int LPR = HD / 8, RPI = 64 / LPR;
-    const int ch = lane % LPR, first_row = (warp - 2) * (32 / LPR) + lane / LPR;
+    // query rows: LPR lanes a row, 16 bytes each; rows up to the segment's columns are zero
+    constexpr int LPR = HD / 8, RPI = 32 / LPR;
+    const int ch = lane % LPR, first_row = lane / LPR;
     Walk w;
     int prefix_segs = 0;
     for (w.begin(a); w.valid;) {
@@ -1409,7 +1399,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16, t_og = t_o + lane_off + wg * MR;
     uint8_t* prow = gbase + (s_p - base) + wg * T::P + r * 128;
     Stat st;
-    st.slot = reinterpret_cast<long long*>(g_stat + wg * T::STAT);
+    st.slot = reinterpret_cast<int*>(g_stat + wg * T::STAT);
     st.red = reinterpret_cast<float*>(st.slot + 2 * MR);
     st.m = st.red + 4 * MR;
     st.alpha = st.m + 2 * MR;
@@ -1427,12 +1417,10 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
       const Cursor s = w.s;
       const bool mine0 = (k & 1) == wg;               // the segment's first tile is this group's
       const bool part = mine0 || !w.last_of_segment();  // the segment has a tile of this group
-      if (part && r < s.rn) st.slot[buf * MR + r] = partial_slot(a, s, w.line, mine0 ? 0 : 1, r);
-      if constexpr (F8) {
-        const QPlace q(a, w.line, w.seg);
+      if (part && r < s.rn) st.slot[buf * MR + r] = (int)partial_slot(a, s, w.line, mine0 ? 0 : 1, r);
+      const QPlace q(a, w.line, w.seg);
+      if (F8 && !part) {  // its factors are not read by this group
         wait(bar_q + 8 * q.bar, q.parity);
-        if (r < q.rows) st.c[r] = q_factor[q.row0 + r];
-        group_sync(wg);
         if (r == 0) mbar_arrive(bar_qfree + 8 * q.bar);
       }
       float l[MR];
@@ -1449,6 +1437,15 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
         wait(bar_s + 8 * sb, (k >> 2) & 1);
         tc_fence_after();
         const uint32_t t_s = tmem + lane_off + sb * MR;
+        if (first) {
+          if (F8) {
+            wait(bar_q + 8 * q.bar, q.parity);
+            if (r < q.rows) st.c[r] = q_factor[q.row0 + r];
+          }
+          if ((warp & 3) == 0) refer<F8>(t_s, columns(s.rn), a.scale_log2, sm, q_factor + q.row0);
+          group_sync(wg);
+          if (F8 && r == 0) mbar_arrive(bar_qfree + 8 * q.bar);
+        }
         uint32_t p[MR / 2];
         if (s.rn <= 16) Softmax<HD, F8, 16>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
         else if (s.rn <= 32) Softmax<HD, F8, 32>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
@@ -1482,7 +1479,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
         if (r < s.rn) {
           const float m = sm[r] == kNoMax ? -INFINITY : sm[r];
           const float sum = (st.red[r] + st.red[MR + r]) + (st.red[2 * MR + r] + st.red[3 * MR + r]);
-          *reinterpret_cast<float2*>(a.part_ml + st.slot[buf * MR + r] * 2) = make_float2(m, sum);
+          *reinterpret_cast<float2*>(a.part_ml + (long long)st.slot[buf * MR + r] * 2) = make_float2(m, sum);
         }
         left = s.rn;
         buf ^= 1;
@@ -1501,10 +1498,10 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
       if (s.begin(a, line)) tiles += s.x1 - s.x;
     int nk = 0, nv = 0;
     for (int e = 0; e < 2 * tiles; ++e) {
-      const bool is_k = e == 0 || ((e & 1) && nk < tiles);  // the order of the loads
-      const int ri = e % T::RN, i = is_k ? nk % T::KN : nv % T::VN;
+      const bool is_k = e == 0 || ((e & 1) && nk < tiles);  // K_0, K_1, V_0, K_2, V_1, ...
+      const int c = is_k ? nk : nv, ri = c % T::RN + (is_k ? 0 : T::RN), i = is_k ? c % T::KN : c % T::VN;
       const uint32_t full = (is_k ? bar_k : bar_v) + 8 * i, free = (is_k ? bar_kfree : bar_vfree) + 8 * i;
-      if (!wait(bar_r + 8 * ri, (e / T::RN) & 1) || !wait(free, ((is_k ? nk / T::KN : nv / T::VN) & 1) ^ 1)) break;
+      if (!wait(bar_r + 8 * ri, (c / T::RN) & 1) || !wait(free, ((is_k ? c / T::KN : c / T::VN) & 1) ^ 1)) break;
       ++(is_k ? nk : nv);
       const uint8_t* src = gbase + (s_r - base) + ri * R::BYTES;
       uint8_t* dst = gbase + ((is_k ? s_k : s_v) - base) + i * E::BYTES;
@@ -1591,15 +1588,15 @@ shared_prefix_combine_kernel(const int* __restrict__ plan, int ctas, int subs, i
   for (int d = 0; d < V; ++d) po[d] = __float2bfloat16_rn(o[d] * inv);
 }
 
-// 4-D map of a cache: [128-byte spans of a key][pages * block keys][KV heads][dims of a span], boxes of
-// `box` keys of one head; a box of `whole` keys brings every span
-CUtensorMap cache_tmap(const at::Tensor& c, int box, int whole, bool f8) {
+// 4-D map of a cache: [128-byte spans of a key][pages * block keys][KV heads][dims of a span], boxes of one
+// span of `box` keys of one head
+CUtensorMap cache_tmap(const at::Tensor& c, int box, bool f8) {
   CUtensorMap m;
   const int hd = c.size(3), nkv = c.size(2), elt = f8 ? 1 : 2;
   const int inner = std::min(hd * elt, 128), spans = hd * elt / inner;
   cuuint64_t dims[4] = {(cuuint64_t)(inner / elt), (cuuint64_t)nkv, (cuuint64_t)(c.size(0) * c.size(1)), (cuuint64_t)spans};
   cuuint64_t strides[3] = {(cuuint64_t)hd * elt, (cuuint64_t)nkv * hd * elt, (cuuint64_t)inner};
-  cuuint32_t bx[4] = {(cuuint32_t)(inner / elt), 1u, (cuuint32_t)box, box == whole ? (cuuint32_t)spans : 1u};
+  cuuint32_t bx[4] = {(cuuint32_t)(inner / elt), 1u, (cuuint32_t)box, 1u};
   cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
   const CUtensorMapSwizzle sw = inner == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
@@ -1704,6 +1701,7 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
   if (q.stride(2) != 1 || q.stride(1) % 8 || q.stride(0) % 8) q = q.contiguous();
   if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 16) q = q.clone(at::MemoryFormat::Contiguous);
   const long long slots = 4 * B * nq + 4LL * p.ctas * sp::MR;
+  RLB_CHECK(slots < (1LL << 31), "shared_prefix_attn: too many rows");
   auto part = at::empty({slots * (hd + 2)}, q.options().dtype(at::kFloat));
   sp::Args a;
   a.q = (const sp::bf16*)q.data_ptr();
@@ -1729,8 +1727,8 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
   a.part_ml = a.part_o + slots * hd;
   CUtensorMap tk = {}, tv = {};
   if (a.box) {
-    tk = sp::cache_tmap(k_cache, a.box, p.tile, f8);
-    tv = sp::cache_tmap(v_cache, a.box, p.tile, f8);
+    tk = sp::cache_tmap(k_cache, a.box, f8);
+    tv = sp::cache_tmap(v_cache, a.box, f8);
   }
   auto launch = [&](auto hdv, auto f8v) {
     constexpr int HD = decltype(hdv)::value;
