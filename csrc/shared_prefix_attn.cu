@@ -37,6 +37,7 @@ constexpr int MR = 64;        // query rows of a prefix unit
 constexpr int kMaxHeads = 64; // query heads per KV head
 constexpr int kUnitInts = 8;  // first tile, tiles, first key, keys' end, table row, first row, first query row, query rows
 constexpr int kRowInts = 4;   // group's first unit (-1: none), group's first row, whether the row has keys
+constexpr int kStart = 1;     // what the start and end of a unit count for on the line, in tiles
 constexpr int kHeader = 8;    // prefix: tiles per CTA, tiles in all; suffix: the same
 
 __device__ int g_shared_prefix_error = 0;
@@ -142,7 +143,7 @@ shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __res
   }
   __syncthreads();
   // prefix units: per group, ceil(rows * Gq / MR) chunks of its query rows
-  int unit_carry = 0, prefix_tiles = 0;
+  int unit_carry = 0, prefix_places = 0;
   for (int g0 = 0; g0 < G; g0 += kPlanThreads) {
     const int g = g0 + tid;
     int chunks = 0, n = 0, start = 0, rows = 0;
@@ -152,29 +153,30 @@ shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __res
       n = (s_share[g] + tile - 1) / tile;
       chunks = n > 0 ? (rows + MR - 1) / MR : 0;
     }
-    // both sums in one scan: units in the high half, tiles in the low one
-    const long long end = block_scan<false>(((long long)chunks << 32) + chunks * n, s_warp2);
-    const int u0 = unit_carry + (int)(end >> 32) - chunks, a0 = prefix_tiles + (int)end - chunks * n;
+    // both sums in one scan: units in the high half, places on the line in the low one
+    const int places = n + kStart;
+    const long long end = block_scan<false>(((long long)chunks << 32) + chunks * places, s_warp2);
+    const int u0 = unit_carry + (int)(end >> 32) - chunks, a0 = prefix_places + (int)end - chunks * places;
     if (g < G) s_unit0[g] = u0;
     for (int c = 0; c < chunks; ++c) {
       int4* m = reinterpret_cast<int4*>(unit + (u0 + c) * kUnitInts);
-      s_first[u0 + c] = a0 + c * n;
-      m[0] = make_int4(a0 + c * n, n, 0, s_share[g]);
+      s_first[u0 + c] = a0 + c * places;
+      m[0] = make_int4(a0 + c * places, n, 0, s_share[g]);
       m[1] = make_int4(s_leader[g], start, c * MR, min(MR, rows - c * MR));
     }
     __syncthreads();
     if (tid == kPlanThreads - 1) s_warp2[0] = end;
     __syncthreads();
     unit_carry += (int)(s_warp2[0] >> 32);
-    prefix_tiles += (int)s_warp2[0];
+    prefix_places += (int)s_warp2[0];
     __syncthreads();
   }
   for (int u = unit_carry + tid; u < nc_max; u += kPlanThreads) {  // unused prefix units
-    s_first[u] = prefix_tiles;
-    *reinterpret_cast<int4*>(unit + u * kUnitInts) = make_int4(prefix_tiles, 0, 0, 0);
+    s_first[u] = prefix_places;
+    *reinterpret_cast<int4*>(unit + u * kUnitInts) = make_int4(prefix_places, 0, 0, 0);
   }
   // suffix units: row b's keys behind its group's shared ones
-  int suffix_tiles = 0;
+  int suffix_places = 0;
   for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     int k0 = 0, k1 = 0, u0 = -1, start = 0;
@@ -188,10 +190,11 @@ shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __res
       }
     }
     const int n = (k1 - k0 + tile - 1) / tile;
-    const int end = block_scan<false>(n, s_warp);
+    const int places = n > 0 ? n + kStart : 0;
+    const int end = block_scan<false>(places, s_warp);
     if (b < B) {
       int4* m = reinterpret_cast<int4*>(unit + (nc_max + b) * kUnitInts);
-      const int a0 = suffix_tiles + end - n;
+      const int a0 = suffix_places + end - places;
       s_first[nc_max + b] = a0;
       m[0] = make_int4(a0, n, k0, k1);
       m[1] = make_int4(b, b, 0, Gq);
@@ -200,10 +203,10 @@ shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __res
     __syncthreads();
     if (tid == kPlanThreads - 1) s_warp[0] = end;
     __syncthreads();
-    suffix_tiles += s_warp[0];
+    suffix_places += s_warp[0];
     __syncthreads();
   }
-  const long long total0 = (long long)prefix_tiles * nkv, total1 = (long long)suffix_tiles * nkv;
+  const long long total0 = (long long)prefix_places * nkv, total1 = (long long)suffix_places * nkv;
   const int per0 = max((int)((total0 + ctas - 1) / ctas), 1), per1 = max((int)((total1 + ctas - 1) / ctas), 1);
   if (tid == 0) *reinterpret_cast<int4*>(plan) = make_int4(per0, (int)total0, per1, (int)total1);
   // every CTA's first unit of each line: the last one that starts at or before its first tile
@@ -345,16 +348,21 @@ struct Cursor {
     u = a.plan[kHeader + line * a.ctas + blockIdx.x];
     load();
     const int y = x - unit[u * kUnitInts] * nkv;
-    kvh = y / n;
-    j = y - kvh * n;
-    return true;
+    kvh = y / (n + kStart);
+    j = y - kvh * (n + kStart) - kStart;
+    if (j < 0) {  // the run begins in the unit's starting places: at its first tile, if that is in the run
+      x -= j;
+      j = 0;
+    }
+    return x < x1;
   }
   // to the next tile; true when it belongs to the same segment (unit, KV head and run)
   __device__ __forceinline__ bool next() {
-    const bool more = ++x < x1;
-    if (++j < n) return more;
+    ++x;
+    if (++j < n) return x < x1;
     j = 0;
-    if (++kvh < nkv || !more) return false;
+    x += kStart;
+    if (++kvh < nkv || x >= x1) return false;
     kvh = 0;
     do {
       if (++u >= u_end) return false;
@@ -956,6 +964,15 @@ __device__ __forceinline__ bool group_any(int wg, bool x) {
       : "memory");
   return r != 0;
 }
+__device__ __forceinline__ bool mbar_poll(uint32_t addr, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(addr), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ float warp_max_f32(float x) {
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;\n" : "=f"(r) : "f"(x));
@@ -975,7 +992,7 @@ struct Walk {
       valid = s.begin(a, 1);
     }
   }
-  __device__ __forceinline__ bool last_of_segment() const { return s.j + 1 == s.n || s.x + 1 == s.x1; }
+  __device__ __forceinline__ bool last_of_segment() const { return s.j + 1 == s.n || s.x + 1 >= s.x1; }
   // to the next tile; true when it belongs to the same segment
   __device__ __forceinline__ bool next(const Args& a) {
     ++t;
@@ -1276,13 +1293,9 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
     uint32_t kph = 0, vph = 0;
     uint32_t info = 0;               // of tile i, at bits 8 (i & 3): columns / 8, and 16 when O is added to
     QPlace q(a, w.line, w.seg);
-    auto issue_s = [&] {
-      if (w.t == 0) {
-        q = QPlace(a, w.line, w.seg);
-        if (!wait(bar_q + 8 * q.bar, q.parity)) return false;
-      }
-      // the buffer of S is free: P of tile ka - 4 was awaited
-      if (!wait(bar_k + 8 * ki, kph)) return false;
+    bool q_ready = false;
+    auto ready = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_poll(bar, parity)); };
+    auto issue_s = [&] {  // S of the walk's tile; its buffer is free: P of tile ka - 4 was awaited
       tc_fence_after();
       const int sb = ka & 3;
       const uint32_t n8 = columns(w.s.rn) >> 3, id = T::FMT | (n8 << 17);
@@ -1300,18 +1313,16 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
       }
       __syncwarp();
       info = (info & ~(0xffu << (8 * sb))) | ((n8 | (w.t >= 2 ? 16u : 0u)) << (8 * sb));
-      w.next(a);
+      if (!w.next(a) && w.valid) {
+        q = QPlace(a, w.line, w.seg);
+        q_ready = false;
+      }
       ++ka;
       if (++ki == T::KN) ki = 0, kph ^= 1;
-      return true;
     };
-    bool ok = true;
-    while (ok && w.valid && ka < 2) ok = issue_s();
-    for (int k = 0; ok && k < ka; ++k) {
-      const int wg = k & 1;
-      ok = wait(bar_v + 8 * vi, vph) && wait(bar_p + 8 * wg, (k >> 1) & 1);
-      if (!ok) break;
+    auto issue_o = [&](int k) {  // O += V P of tile k
       tc_fence_after();
+      const int wg = k & 1;
       const uint32_t i = info >> (8 * (k & 3)), id = T::FMT | (1u << 15) | (1u << 16) | ((i & 15u) << 17);
       const uint32_t vd = desc_lo(s_v + vi * E::BYTES, HD == 128 ? 128 * 128 : 0), pd = desc_lo(s_p + wg * T::P, 0);
       if (elect_one()) {
@@ -1323,7 +1334,36 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
       }
       __syncwarp();
       if (++vi == T::VN) vi = 0, vph ^= 1;
-      if (w.valid) ok = issue_s();
+    };
+    // whichever of the two products has its operands is issued: S up to two tiles ahead of O
+    int idle = 0;
+    long long since = 0;
+    for (int k = 0; k < ka || w.valid;) {
+      bool progress = false;
+      if (w.valid && ka <= k + 2) {
+        if (!q_ready) q_ready = ready(bar_q + 8 * q.bar, q.parity);
+        if (q_ready && ready(bar_k + 8 * ki, kph)) {
+          issue_s();
+          progress = true;
+        }
+      }
+      if (k < ka && ready(bar_p + 8 * (k & 1), (k >> 1) & 1) && ready(bar_v + 8 * vi, vph)) {
+        issue_o(k);
+        ++k;
+        progress = true;
+      }
+      if (progress) {
+        idle = 0;
+      } else if ((++idle & 63) == 0) {  // bounded: look at the clock now and then
+        if (__any_sync(0xffffffffu, *abort_flag)) break;
+        const long long now = clock64();
+        if (idle == 64) {
+          since = now;
+        } else if (now - since > kWaitCycles) {
+          atomicExch(&g_shared_prefix_error, kErrWait);
+          *abort_flag = 1;
+        }
+      }
     }
   } else {
     // query rows: LPR lanes a row, 16 bytes each; rows up to the segment's columns are zero
@@ -1346,43 +1386,32 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
         return a.q + (long long)(w.s.row0 + b) * a.q_row + (long long)(w.s.kvh * a.Gq + h) * a.q_head + ch * 8;
       };
       const uint32_t at = q.row0 * (HD * 2) + (ch >> 3) * (q.rows * 128);
-      if constexpr (!F8) {
-        for (int r = first_row; r < rows; r += RPI)
-          cp_async16_or_zero(s_q + at + r * 128 + (((ch & 7) ^ (r & 7)) << 4), r < w.s.rn ? src(r) : a.q, r < w.s.rn);
-        asm volatile("cp.async.wait_all;\n" ::: "memory");
-      } else {
-        constexpr int U = 4;  // rows in flight a lane
-        for (int r0 = first_row; r0 < rows; r0 += U * RPI) {
-          uint4 v[U];
+      auto place = [&](int r) { return at + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
+      for (int r = first_row; r < rows; r += RPI)
+        cp_async16_or_zero(s_q + place(r), r < w.s.rn ? src(r) : a.q, r < w.s.rn);
+      asm volatile("cp.async.wait_all;\n" ::: "memory");
+      if constexpr (F8) {  // to f16, each lane the 16 bytes that it brought
+#pragma unroll 2
+        for (int r = first_row; r < rows; r += RPI) {
+          uint4 v = *reinterpret_cast<const uint4*>(gbase + place(r));
+          uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+          float mx = 0.f;
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            v[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (r0 + u * RPI < w.s.rn) v[u] = *reinterpret_cast<const uint4*>(src(r0 + u * RPI));
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x[i]));
+            mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
           }
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * RPI;
-            uint32_t* x = reinterpret_cast<uint32_t*>(&v[u]);
-            float mx = 0.f;
+          for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const int ex = f16_row_exponent(mx);
+          const float f = f16_row_factor(ex);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x[i]));
-              mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-#pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const int ex = f16_row_exponent(mx);
-            const float f = f16_row_factor(ex);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 g = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x[i]));
-              x[i] = pack_f16(g.x * f, g.y * f);
-            }
-            if (r < rows) {
-              if (ch == 0) q_factor[q.row0 + r] = a.scale_log2 * f16_row_inverse(ex);
-              *reinterpret_cast<uint4*>(gbase + at + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v[u];
-            }
+          for (int i = 0; i < 4; ++i) {
+            const float2 g = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x[i]));
+            x[i] = pack_f16(g.x * f, g.y * f);
           }
+          if (ch == 0) q_factor[q.row0 + r] = a.scale_log2 * f16_row_inverse(ex);
+          *reinterpret_cast<uint4*>(gbase + place(r)) = v;
         }
       }
       fence_async();
@@ -1492,10 +1521,9 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
     const int tid = threadIdx.x - 384;
     constexpr int CH = HD / 16;  // chunks of 16 values of a key
-    Cursor s;
+    Walk w;
     int tiles = 0;
-    for (int line = 0; line < 2; ++line)
-      if (s.begin(a, line)) tiles += s.x1 - s.x;
+    for (w.begin(a); w.valid; w.next(a)) ++tiles;
     int nk = 0, nv = 0;
     for (int e = 0; e < 2 * tiles; ++e) {
       const bool is_k = e == 0 || ((e & 1) && nk < tiles);  // K_0, K_1, V_0, K_2, V_1, ...
@@ -1566,7 +1594,7 @@ shared_prefix_combine_kernel(const int* __restrict__ plan, int ctas, int subs, i
   auto add_unit = [&](int line, int u, int local) {
     const int n = unit[u * kUnitInts + 1], per = plan[2 * line];
     if (n == 0) return;
-    const int x = unit[u * kUnitInts] * nkv + kvh * n;
+    const int x = unit[u * kUnitInts] * nkv + kvh * (n + kStart) + kStart;
     for (int c = x / per; c <= (x + n - 1) / per; ++c) {
       const int tiles = min(x + n, (c + 1) * per) - max(x, c * per);
       for (int sub = 0; sub < min(subs, tiles); ++sub) {
