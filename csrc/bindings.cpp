@@ -53,7 +53,8 @@ std::tuple<int64_t, int64_t> copy_cache_pages(at::Tensor cache, std::vector<int6
 at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, at::Tensor seq_lens, int64_t nq,
                               int64_t nkv, int64_t hd, int64_t block);
 at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor block_tables,
-                              at::Tensor plan, int64_t groups, double scale, double k_scale, double v_scale);
+                              at::Tensor seq_lens, at::Tensor group_starts, at::Tensor prefix_lens,
+                              c10::optional<at::Tensor> given, double scale, double k_scale, double v_scale);
 int64_t shared_prefix_error_flag(bool reset);
 // gemm_tcgen05.cu
 at::Tensor gemm_nt(at::Tensor a, at::Tensor b);
@@ -190,7 +191,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_decode_attn", &paged_decode_attn);
   m.def("copy_cache_pages", &copy_cache_pages, "copies of KV-cache pages in every layer, page lists on the host");
   m.def("shared_prefix_plan", &shared_prefix_plan, "work plan of shared_prefix_attn for one decode step");
-  m.def("shared_prefix_attn", &shared_prefix_attn, "paged decode attention, the prefix of a group read once");
+  m.def("shared_prefix_attn", &shared_prefix_attn, "paged decode attention, the prefix of a group read once (planned unless a plan is given)");
   m.def("shared_prefix_error_flag", &shared_prefix_error_flag, py::arg("reset") = false,
         "error word: 1 group bounds, 2 block-table entry outside the cache, 3 expired wait");
   m.def("gemm_nt", &gemm_nt);

@@ -165,6 +165,36 @@ struct alignas(8 * sizeof(T)) Vec8 {
   }
 };
 
+// Sums and magnitudes on packed pairs (a sum of two 8- or 11-bit mantissas is rounded once either way, as in
+// fp32 and then to T); scalars for fp32.
+template <typename T>
+__device__ __forceinline__ void add8(Vec8<T>& a, const Vec8<T>& b) {
+  if constexpr (sizeof(T) == 2) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<T2*>(a.v)[i] = __hadd2_rn(reinterpret_cast<T2*>(a.v)[i], reinterpret_cast<const T2*>(b.v)[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a.v[i] += b.v[i];
+  }
+}
+template <typename T>
+__device__ __forceinline__ float amax8(const Vec8<T>& a) {
+  if constexpr (sizeof(T) == 2) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* p = reinterpret_cast<const T2*>(a.v);
+    const T2 m = __hmax2(__hmax2(__habs2(p[0]), __habs2(p[1])), __hmax2(__habs2(p[2]), __habs2(p[3])));
+    const float r = fmaxf(to_f(m.x), to_f(m.y));
+    return r == r ? r : 0.f;  // as fmaxf: a NaN counts for nothing
+  } else {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(a.v[i]));
+    return m;
+  }
+}
+
 template <typename T, int NV, int TPR>
 __global__ void __launch_bounds__(128)
 rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* __restrict__ w,
@@ -197,9 +227,7 @@ rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T
     const int j = t + k * TPR;
     if (j < nv) {
       if (dr) {
-        const Vec8<T> d = dr[j];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[k].v[i] = from_f<T>(to_f(f[k].v[i]) + to_f(d.v[i]));
+        add8(f[k], dr[j]);
         sr[j] = f[k];
       }
 #pragma unroll
@@ -222,10 +250,8 @@ rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T
     if (j < nv) {
       const Vec8<T> g = wr[j];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        f[k].v[i] = from_f<T>(to_f(f[k].v[i]) * r * to_f(g.v[i]));
-        amax[k] = fmaxf(amax[k], fabsf(to_f(f[k].v[i])));
-      }
+      for (int i = 0; i < 8; ++i) f[k].v[i] = from_f<T>(to_f(f[k].v[i]) * r * to_f(g.v[i]));
+      amax[k] = amax8(f[k]);
       f[k].keep();
     }
   }

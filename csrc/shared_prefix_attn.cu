@@ -1081,13 +1081,15 @@ struct Softmax {
   static __device__ __forceinline__ void tile(int wg, uint32_t t_s, uint32_t t_o, bool live, bool first, float scale,
                                               const Stat& st, float* sm, float* l, uint32_t* p, int r, W wait_o) {
     const int warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-    if (group_any(wg, weights(p, t_s, live, scale, sm, st.c) > kMost)) {
+    // after one round every value is at most 1
+#pragma unroll 1
+    while (group_any(wg, weights(p, t_s, live, scale, sm, st.c) > kMost)) {
+#pragma unroll 1
+      for (int h = 0; h < N; h += 16) {
+        float y[16];
+        tmem_load<16>(t_s + h, y);
 #pragma unroll
-      for (int h = 0; h < N; h += H) {
-        float y[H];
-        tmem_load<H>(t_s + h, y);
-#pragma unroll
-        for (int i = 0; i < H; ++i) {
+        for (int i = 0; i < 16; ++i) {
           const float mx = warp_max_f32(live ? y[i] * (F8 ? st.c[h + i] : scale) : -INFINITY);
           if (lane == i) st.red[warp4 * MR + h + i] = mx;
         }
@@ -1104,21 +1106,18 @@ struct Softmax {
       if (!first) {
         wait_o();
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < N; h += 16) {
           float o[16];
           tmem_load<16>(t_o + h, o);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float f = st.alpha[h + i];
-            o[i] *= f;
-            l[h + i] *= f;
-          }
+          for (int i = 0; i < 16; ++i) o[i] *= st.alpha[h + i];
           tmem_st16(t_o + h, o);
         }
         asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < N; ++i) l[i] *= st.alpha[i];
       }
-      weights(p, t_s, live, scale, sm, st.c);
     }
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
@@ -1669,10 +1668,11 @@ using namespace rlb;
 // [group_starts[g], group_starts[g+1]), of whose keys the first prefix_lens[g] are the same
 at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, at::Tensor seq_lens, int64_t nq,
                               int64_t nkv, int64_t hd, int64_t block) {
-  for (const at::Tensor& t : {group_starts, prefix_lens, seq_lens})
-    RLB_CHECK(t.is_cuda() && t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous() &&
-                  t.device() == seq_lens.device(),
-              "shared_prefix_plan: contiguous int32 vectors on one CUDA device expected");
+  for (at::Tensor* t : {&group_starts, &prefix_lens, &seq_lens}) {
+    RLB_CHECK(t->is_cuda() && t->dim() == 1 && t->device() == seq_lens.device(),
+              "shared_prefix_plan: integer vectors on one CUDA device expected");
+    if (t->scalar_type() != at::kInt || !t->is_contiguous()) *t = t->to(at::kInt).contiguous();
+  }
   const int64_t G = prefix_lens.size(0), B = seq_lens.size(0);
   RLB_CHECK(group_starts.size(0) == G + 1, "shared_prefix_plan: group_starts needs one entry more than prefix_lens");
   RLB_CHECK(nkv >= 1 && nq >= nkv && nq % nkv == 0 && nq / nkv <= sp::kMaxHeads,
@@ -1694,8 +1694,10 @@ at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, a
   return plan;
 }
 
+// planned here unless `given` holds the plan of these lengths
 at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor block_tables,
-                              at::Tensor plan, int64_t groups, double scale, double k_scale, double v_scale) {
+                              at::Tensor seq_lens, at::Tensor group_starts, at::Tensor prefix_lens,
+                              c10::optional<at::Tensor> given, double scale, double k_scale, double v_scale) {
   RLB_CHECK(q.is_cuda() && q.dim() == 3 && q.scalar_type() == at::kBFloat16,
             "shared_prefix_attn: q must be bf16 [rows, heads, dims]");
   const bool f8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
@@ -1709,23 +1711,29 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
   RLB_CHECK(k_cache.size(3) == hd && nkv >= 1 && nq >= nkv && nq % nkv == 0 && nq / nkv <= sp::kMaxHeads,
             "shared_prefix_attn: heads of q and cache do not match");
   RLB_CHECK(nb >= 1 && bs >= 1 && nb * bs < (1LL << 31), "shared_prefix_attn: the cache needs 1 to 2^31 - 1 keys");
-  RLB_CHECK(block_tables.is_cuda() && block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt &&
-                block_tables.is_contiguous() && block_tables.size(0) == B && (B == 0 || block_tables.size(1) >= 1),
-            "shared_prefix_attn: int32 block tables [rows, pages] expected");
+  RLB_CHECK(block_tables.is_cuda() && block_tables.dim() == 2 && block_tables.size(0) == B &&
+                (B == 0 || block_tables.size(1) >= 1),
+            "shared_prefix_attn: block tables [rows, pages] expected");
+  RLB_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == B, "shared_prefix_attn: a length for every row expected");
+  if (block_tables.scalar_type() != at::kInt || !block_tables.is_contiguous())
+    block_tables = block_tables.to(at::kInt).contiguous();
+  const int64_t groups = prefix_lens.size(0);
   const int Gq = nq / nkv;
   const bool tc = sp::use_tc(hd, bs);
   const sp::Shape p = sp::shape_of(tc);
   const int units = sp::max_chunks(B, groups, Gq) + B;
-  RLB_CHECK(plan.is_cuda() && plan.scalar_type() == at::kInt && plan.is_contiguous() && groups >= 0 &&
-                plan.numel() == sp::plan_ints(p, units, B),
-            "shared_prefix_attn: the plan is of another batch");
-  for (const at::Tensor& t : {k_cache, v_cache, block_tables, plan})
+  for (const at::Tensor& t : {k_cache, v_cache, block_tables, seq_lens})
     RLB_CHECK(t.device() == q.device(), "shared_prefix_attn: all tensors must be on one device");
   for (const at::Tensor& t : {k_cache, v_cache})
     RLB_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "shared_prefix_attn: caches must be 16-byte aligned");
   const c10::cuda::CUDAGuard guard(q.device());
   auto out = at::empty({B, nq, hd}, q.options());
   if (B == 0) return out;
+  const bool planned = given.has_value() && given->defined();
+  at::Tensor plan = planned ? *given : shared_prefix_plan(group_starts, prefix_lens, seq_lens, nq, nkv, hd, bs);
+  RLB_CHECK(plan.is_cuda() && plan.scalar_type() == at::kInt && plan.is_contiguous() && plan.device() == q.device() &&
+                plan.numel() == sp::plan_ints(p, units, B),
+            "shared_prefix_attn: the plan is of another batch");
   if (q.stride(2) != 1 || q.stride(1) % 8 || q.stride(0) % 8) q = q.contiguous();
   if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 16) q = q.clone(at::MemoryFormat::Contiguous);
   const long long slots = 4 * B * nq + 4LL * p.ctas * sp::MR;

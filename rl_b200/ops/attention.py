@@ -27,7 +27,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from rl_b200.ops._ext import ext, use_native
+from rl_b200.ops._ext import add_launches, ext, use_native
 
 __all__ = [
     "flash_attn_varlen",
@@ -240,11 +240,12 @@ class SharedPrefixPlan(NamedTuple):
 
 
 def _check_groups(seq_lens, group_starts, prefix_lens):
-    for name, t in (("seq_lens", seq_lens), ("group_starts", group_starts), ("prefix_lens", prefix_lens)):
-        if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.device != seq_lens.device:
-            raise ValueError(f"shared prefix: {name} must be an integer vector on {seq_lens.device}, got "
-                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    if group_starts.numel() != prefix_lens.numel() + 1:
+    dev = seq_lens.device
+    for t in (seq_lens, group_starts, prefix_lens):
+        if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.device != dev:
+            raise ValueError("shared prefix: lengths and group starts must be integer vectors on one device, got "
+                             f"{tuple(t.shape)} {t.dtype} on {t.device} (lengths on {dev})")
+    if group_starts.shape[0] != prefix_lens.shape[0] + 1:
         raise ValueError(f"shared prefix: {prefix_lens.numel()} prefix lengths need {prefix_lens.numel() + 1} group "
                          f"starts, got {group_starts.numel()}")
 
@@ -257,9 +258,9 @@ def shared_prefix_plan(seq_lens, group_starts, prefix_lens, num_heads: int, num_
     device, without a synchronisation), so one plan serves every layer of the step; lengths that
     change need a new one.  GPU only."""
     _check_groups(seq_lens, group_starts, prefix_lens)
-    i32 = [t.to(torch.int32).contiguous() for t in (group_starts, prefix_lens, seq_lens)]
     key = (int(num_heads), int(num_kv_heads), int(head_dim), int(block_size))
-    return SharedPrefixPlan(ext().shared_prefix_plan(*i32, *key), seq_lens.numel(), prefix_lens.numel(), *key)
+    return SharedPrefixPlan(ext().shared_prefix_plan(group_starts, prefix_lens, seq_lens, *key), seq_lens.shape[0],
+                            prefix_lens.shape[0], *key)
 
 
 def shared_prefix_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, group_starts, prefix_lens,
@@ -286,9 +287,9 @@ def shared_prefix_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, 
             or k_cache.shape[2] == 0 or q.shape[1] % k_cache.shape[2]:
         raise ValueError(f"shared prefix attention: q {tuple(q.shape)} with caches {tuple(k_cache.shape)}, "
                          f"{tuple(v_cache.shape)}")
-    if block_tables.dim() != 2 or block_tables.shape[0] != B or seq_lens.numel() != B:
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or seq_lens.shape[0] != B:
         raise ValueError(f"shared prefix attention: {B} queries, block tables {tuple(block_tables.shape)}, "
-                         f"{seq_lens.numel()} lengths")
+                         f"{seq_lens.shape[0]} lengths")
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if not use_native(q):
         if k_cache.dtype == torch.float8_e4m3fn:
@@ -298,11 +299,12 @@ def shared_prefix_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, 
         if bool(live.any()):  # every row's table is complete: the grouping changes what is read, not the result
             out[live] = paged_decode_attention_ref(q[live], k_cache, v_cache, block_tables[live], seq_lens[live], scale)
         return out
-    key = (q.shape[1], k_cache.shape[2], q.shape[2], k_cache.shape[1])
-    if plan is None:
-        plan = shared_prefix_plan(seq_lens, group_starts, prefix_lens, *key)
-    elif plan[1:] != (B, prefix_lens.numel(), *key):
+    if plan is not None and plan[1:] != (B, prefix_lens.shape[0], q.shape[1], k_cache.shape[2], q.shape[2],
+                                         k_cache.shape[1]):
         raise ValueError("shared prefix attention: a plan for (rows, groups, heads, KV heads, head dim, block size) "
-                         f"{plan[1:]} used for {(B, prefix_lens.numel(), *key)}")
-    return ext().shared_prefix_attn(q, k_cache, v_cache, block_tables.to(torch.int32).contiguous(), plan.buf,
-                                    plan.groups, float(scale), float(k_scale), float(v_scale))
+                         f"{plan[1:]} used for {B} rows, {prefix_lens.shape[0]} groups, q {tuple(q.shape)}, caches "
+                         f"{tuple(k_cache.shape)}")
+    if plan is None:
+        add_launches(1)  # the native call plans first
+    return ext().shared_prefix_attn(q, k_cache, v_cache, block_tables, seq_lens, group_starts, prefix_lens,
+                                    None if plan is None else plan.buf, scale, k_scale, v_scale)

@@ -95,29 +95,28 @@ def add_rms_norm(x: torch.Tensor, delta: torch.Tensor, w: torch.Tensor, eps: flo
     return add_rms_norm_ref(x, delta, w, eps)
 
 
-def _norm_fp8(x: torch.Tensor, delta, w: torch.Tensor, eps: float, mx: bool):
-    H = x.shape[-1]
-    if x.dim() < 1 or H % 128 or H == 0:
+def _check_norm_fp8(x: torch.Tensor, delta, w: torch.Tensor) -> None:
+    H = x.shape[-1] if x.dim() else 0
+    if H == 0 or H % 128:
         raise ValueError(f"rms_norm_fp8: the hidden size must be a multiple of 128, got shape {tuple(x.shape)}")
-    if w.shape != (H,) or w.dtype != x.dtype or w.device != x.device:
+    if w.dim() != 1 or w.shape[0] != H or w.dtype != x.dtype or w.device != x.device:
         raise ValueError(f"rms_norm_fp8: weight {tuple(w.shape)} {w.dtype} on {w.device} for input "
                          f"{tuple(x.shape)} {x.dtype} on {x.device}")
     if delta is not None and (delta.shape != x.shape or delta.dtype != x.dtype or delta.device != x.device):
         raise ValueError(f"rms_norm_fp8: delta {tuple(delta.shape)} {delta.dtype} on {delta.device} for input "
                          f"{tuple(x.shape)} {x.dtype} on {x.device}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, delta, w)):
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (delta is not None and delta.requires_grad)):
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad() (rollout only)")
-    if not use_native(x):
-        from rl_b200.ops.fp8_gemm import quant_act_mx
-        from rl_b200.ops.quant import quant_fp8_group_ref
 
-        y, s = (rms_norm_ref(x, w, eps), None) if delta is None else add_rms_norm_ref(x, delta, w, eps)
-        y2 = y.reshape(-1, H)
-        q, sc = quant_act_mx(y2) if mx else quant_fp8_group_ref(y2, 128, False)
-        return q.view(x.shape), sc, s
 
-    out = ext().rmsnorm_fp8(x, delta, w, float(eps), bool(mx), bool(mx))
-    return out if delta is not None else (*out, None)
+def _norm_fp8_ref(x: torch.Tensor, delta, w: torch.Tensor, eps: float, mx: bool):
+    from rl_b200.ops.fp8_gemm import quant_act_mx
+    from rl_b200.ops.quant import quant_fp8_group_ref
+
+    y, s = (rms_norm_ref(x, w, eps), None) if delta is None else add_rms_norm_ref(x, delta, w, eps)
+    y2 = y.reshape(-1, x.shape[-1])
+    q, sc = quant_act_mx(y2) if mx else quant_fp8_group_ref(y2, 128, False)
+    return q.view(x.shape), sc, s
 
 
 def rms_norm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, mx: bool = True):
@@ -129,9 +128,11 @@ def rms_norm_fp8(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, mx: bool =
     :func:`rl_b200.ops.fp8_gemm.gemm_fp8`.  The hidden size is a multiple of 128 (at most 16384 on a
     GPU).  For inference: an input that needs a gradient is refused.
     """
-    return tuple(_norm_fp8(x, None, w, eps, mx)[:2])
+    _check_norm_fp8(x, None, w)
+    return tuple(ext().rmsnorm_fp8(x, None, w, eps, mx, mx)) if x.is_cuda else _norm_fp8_ref(x, None, w, eps, mx)[:2]
 
 
 def add_rms_norm_fp8(x: torch.Tensor, delta: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, mx: bool = True):
     """``(q, scales, x + delta)``: :func:`rms_norm_fp8` of the residual sum, which is returned too."""
-    return tuple(_norm_fp8(x, delta, w, eps, mx))
+    _check_norm_fp8(x, delta, w)
+    return tuple(ext().rmsnorm_fp8(x, delta, w, eps, mx, mx)) if x.is_cuda else _norm_fp8_ref(x, delta, w, eps, mx)
