@@ -196,7 +196,7 @@ __device__ __forceinline__ float amax8(const Vec8<T>& a) {
 }
 
 template <typename T, int NV, int TPR>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, sizeof(T) == 2 && NV <= 16 ? 4 : 1)
 rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T* __restrict__ w,
                    T* __restrict__ s_out, __nv_fp8_e4m3* __restrict__ q, float* __restrict__ scales, int rows, int H,
                    float eps, bool pow2, int ld) {
@@ -222,20 +222,30 @@ rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T
     if (j < nv) f[k] = xr[j];
   }
   float ss = 0.f;
+  // loads of delta (and below of w) go LB at a time: one by one, each would wait for memory
+  constexpr int LB = 4;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int j = t + k * TPR;
-    if (j < nv) {
-      if (dr) {
-        add8(f[k], dr[j]);
-        sr[j] = f[k];
-      }
+  for (int k0 = 0; k0 < NV; k0 += LB) {
+    Vec8<T> d[LB];
+    if (dr)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float v = to_f(f[k].v[i]);
-        ss += v * v;
+      for (int k = 0; k < LB; ++k)
+        if (t + (k0 + k) * TPR < nv) d[k] = dr[t + (k0 + k) * TPR];
+#pragma unroll
+    for (int k = 0; k < LB; ++k) {
+      const int j = t + (k0 + k) * TPR;
+      if (j < nv) {
+        if (dr) {
+          add8(f[k0 + k], d[k]);
+          sr[j] = f[k0 + k];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float v = to_f(f[k0 + k].v[i]);
+          ss += v * v;
+        }
+        f[k0 + k].keep();
       }
-      f[k].keep();
     }
   }
   ss = TPR == 128 ? block_sum(ss, red) : warp_sum(ss);
@@ -244,15 +254,21 @@ rmsnorm_fp8_kernel(const T* __restrict__ x, const T* __restrict__ delta, const T
   // H % 128 == 0: a half-warp's 16 vectors are all inside the row or all outside.
   float amax[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int j = t + k * TPR;
-    amax[k] = 0.f;
-    if (j < nv) {
-      const Vec8<T> g = wr[j];
+  for (int k0 = 0; k0 < NV; k0 += LB) {
+    Vec8<T> g[LB];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[k].v[i] = from_f<T>(to_f(f[k].v[i]) * r * to_f(g.v[i]));
-      amax[k] = amax8(f[k]);
-      f[k].keep();
+    for (int k = 0; k < LB; ++k)
+      if (t + (k0 + k) * TPR < nv) g[k] = wr[t + (k0 + k) * TPR];
+#pragma unroll
+    for (int k = 0; k < LB; ++k) {
+      amax[k0 + k] = 0.f;
+      if (t + (k0 + k) * TPR < nv) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          f[k0 + k].v[i] = from_f<T>(to_f(f[k0 + k].v[i]) * r * to_f(g[k].v[i]));
+        amax[k0 + k] = amax8(f[k0 + k]);
+        f[k0 + k].keep();
+      }
     }
   }
 #pragma unroll
