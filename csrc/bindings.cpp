@@ -51,7 +51,7 @@ std::tuple<int64_t, int64_t> copy_cache_pages(at::Tensor cache, std::vector<int6
                                               std::vector<int64_t> tokens);
 // shared_prefix_attn.cu
 at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, at::Tensor seq_lens, int64_t nq,
-                              int64_t nkv, int64_t hd, int64_t block);
+                              int64_t nkv, int64_t hd, int64_t block, int64_t max_blocks);
 at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor block_tables,
                               at::Tensor seq_lens, at::Tensor group_starts, at::Tensor prefix_lens,
                               c10::optional<at::Tensor> given, double scale, double k_scale, double v_scale);
@@ -193,7 +193,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("shared_prefix_plan", &shared_prefix_plan, "work plan of shared_prefix_attn for one decode step");
   m.def("shared_prefix_attn", &shared_prefix_attn, "paged decode attention, the prefix of a group read once (planned unless a plan is given)");
   m.def("shared_prefix_error_flag", &shared_prefix_error_flag, py::arg("reset") = false,
-        "error word: 1 group bounds, 2 block-table entry outside the cache, 3 expired wait");
+        "error word: 1 group bounds or lengths, 2 block-table entry outside the cache, 3 expired wait");
   m.def("gemm_nt", &gemm_nt);
   m.def("gemm_error_flag", &gemm_error_flag, py::arg("reset") = false);
   m.def("gemm_rs", &gemm_rs);

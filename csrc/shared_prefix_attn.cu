@@ -41,7 +41,7 @@ constexpr int kStart = 1;     // what the start and end of a unit count for on t
 constexpr int kHeader = 8;    // prefix: tiles per CTA, tiles in all; suffix: the same
 
 __device__ int g_shared_prefix_error = 0;
-constexpr int kErrGroups = 1, kErrPage = 2, kErrWait = 3;  // error words
+constexpr int kErrLengths = 1, kErrPage = 2, kErrWait = 3;  // error words
 
 // What differs between the plans of the two kernels: CTAs, keys per tile.
 struct Shape {
@@ -89,7 +89,7 @@ __device__ __forceinline__ int last_at_most(const int* a, int n, int x) {
 __global__ void __launch_bounds__(kPlanThreads)
 shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __restrict__ prefix_lens,
                           const int* __restrict__ seq_lens, int G, int B, int Gq, int nkv, int ctas, int tile,
-                          int* __restrict__ plan) {
+                          int capacity, int* __restrict__ plan) {
   extern __shared__ int s_mem[];
   __shared__ int s_warp[32];
   __shared__ long long s_warp2[32];
@@ -105,11 +105,17 @@ shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __res
   int* cta_unit = plan + kHeader;
   int* unit = plan + unit_offset(ctas);
   int* rowinfo = unit + units * kUnitInts;
-  for (int b = tid; b < B; b += kPlanThreads) s_len[b] = max(seq_lens[b], 0);
+  // lengths are kept inside the block tables, and so short that no place on a line leaves 31 bits
+  const int longest = (int)min((long long)capacity, (long long)max((1 << 30) / (nkv * units), 1) * BT);
+  bool bad = false;
+  for (int b = tid; b < B; b += kPlanThreads) {
+    const int len = max(seq_lens[b], 0);
+    bad |= len > longest;
+    s_len[b] = min(len, longest);
+  }
   for (int g = tid; g < G; g += kPlanThreads) s_share[g] = max(prefix_lens[g], 0);
   // group starts, made ascending and kept inside [0, B]: groups never overlap
   int carry = 0;
-  bool bad = false;
   for (int g0 = 0; g0 <= G; g0 += kPlanThreads) {
     const int g = g0 + tid;
     const int raw = g <= G ? group_starts[g] : 0;
@@ -121,7 +127,7 @@ shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __res
     __syncthreads();
     carry = s_start[min(G, g0 + kPlanThreads - 1)];
   }
-  if (bad) atomicExch(&g_shared_prefix_error, kErrGroups);
+  if (bad) atomicExch(&g_shared_prefix_error, kErrLengths);
   // a group shares what every live row of it has, in multiples of BT; one live row shares nothing
   for (int g = warp; g < G; g += kPlanThreads / 32) {
     int len = s_share[g], live = 0, leader = B;
@@ -1081,9 +1087,10 @@ struct Softmax {
   static __device__ __forceinline__ void tile(int wg, uint32_t t_s, uint32_t t_o, bool live, bool first, float scale,
                                               const Stat& st, float* sm, float* l, uint32_t* p, int r, W wait_o) {
     const int warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-    // after one round every value is at most 1
 #pragma unroll 1
-    while (group_any(wg, weights(p, t_s, live, scale, sm, st.c) > kMost)) {
+    for (int round = 0;; ++round) {
+      const bool over = group_any(wg, weights(p, t_s, live, scale, sm, st.c) > kMost);
+      if (!over || round > 0) break;  // after a round every value is about 1 at most
 #pragma unroll 1
       for (int h = 0; h < N; h += 16) {
         float y[16];
@@ -1667,7 +1674,7 @@ using namespace rlb;
 // int32 plan of the work of one decode step (see the kernel): group g's rows are
 // [group_starts[g], group_starts[g+1]), of whose keys the first prefix_lens[g] are the same
 at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, at::Tensor seq_lens, int64_t nq,
-                              int64_t nkv, int64_t hd, int64_t block) {
+                              int64_t nkv, int64_t hd, int64_t block, int64_t max_blocks) {
   for (at::Tensor* t : {&group_starts, &prefix_lens, &seq_lens}) {
     RLB_CHECK(t->is_cuda() && t->dim() == 1 && t->device() == seq_lens.device(),
               "shared_prefix_plan: integer vectors on one CUDA device expected");
@@ -1677,7 +1684,8 @@ at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, a
   RLB_CHECK(group_starts.size(0) == G + 1, "shared_prefix_plan: group_starts needs one entry more than prefix_lens");
   RLB_CHECK(nkv >= 1 && nq >= nkv && nq % nkv == 0 && nq / nkv <= sp::kMaxHeads,
             "shared_prefix_plan: query heads must be a multiple of the KV heads, at most 64 per KV head");
-  RLB_CHECK(B <= 8192 && G <= 8192 && block >= 1, "shared_prefix_plan: at most 8192 rows and groups");
+  RLB_CHECK(B <= 8192 && G <= 8192 && block >= 1 && max_blocks >= 0, "shared_prefix_plan: at most 8192 rows and groups");
+  const int capacity = (int)std::min<int64_t>(block * std::min<int64_t>(max_blocks, 1LL << 31), (1LL << 31) - 256);
   const c10::cuda::CUDAGuard guard(seq_lens.device());
   const int Gq = nq / nkv;
   const sp::Shape p = sp::shape_of(sp::use_tc(hd, block));
@@ -1689,7 +1697,7 @@ at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, a
     RLB_CUDA_CHECK(cudaFuncSetAttribute(sp::shared_prefix_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   sp::shared_prefix_plan_kernel<<<1, sp::kPlanThreads, smem, stream()>>>(
       group_starts.data_ptr<int>(), prefix_lens.data_ptr<int>(), seq_lens.data_ptr<int>(), G, B, Gq, nkv, p.ctas, p.tile,
-      plan.data_ptr<int>());
+      capacity, plan.data_ptr<int>());
   RLB_CUDA_CHECK(cudaGetLastError());
   return plan;
 }
@@ -1730,7 +1738,8 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
   auto out = at::empty({B, nq, hd}, q.options());
   if (B == 0) return out;
   const bool planned = given.has_value() && given->defined();
-  at::Tensor plan = planned ? *given : shared_prefix_plan(group_starts, prefix_lens, seq_lens, nq, nkv, hd, bs);
+  at::Tensor plan = planned ? *given : shared_prefix_plan(group_starts, prefix_lens, seq_lens, nq, nkv, hd, bs,
+                                                           block_tables.size(1));
   RLB_CHECK(plan.is_cuda() && plan.scalar_type() == at::kInt && plan.is_contiguous() && plan.device() == q.device() &&
                 plan.numel() == sp::plan_ints(p, units, B),
             "shared_prefix_attn: the plan is of another batch");

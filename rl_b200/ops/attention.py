@@ -237,6 +237,7 @@ class SharedPrefixPlan(NamedTuple):
     kv_heads: int
     head_dim: int
     block_size: int
+    max_blocks: int
 
 
 def _check_groups(seq_lens, group_starts, prefix_lens):
@@ -251,14 +252,14 @@ def _check_groups(seq_lens, group_starts, prefix_lens):
 
 
 def shared_prefix_plan(seq_lens, group_starts, prefix_lens, num_heads: int, num_kv_heads: int, head_dim: int,
-                       block_size: int) -> SharedPrefixPlan:
+                       block_size: int, max_blocks: int) -> SharedPrefixPlan:
     """Plan the attention of one decode step: which CTA takes which keys of which rows.
 
-    The plan depends on the lengths and the head and page sizes alone (lengths are read on the
-    device, without a synchronisation), so one plan serves every layer of the step; lengths that
-    change need a new one.  GPU only."""
+    The plan depends on the lengths and the head, page and table sizes alone (lengths are read on
+    the device, without a synchronisation), so one plan serves every layer of the step; lengths that
+    change need a new one.  ``max_blocks`` is the width of the block tables.  GPU only."""
     _check_groups(seq_lens, group_starts, prefix_lens)
-    key = (int(num_heads), int(num_kv_heads), int(head_dim), int(block_size))
+    key = (int(num_heads), int(num_kv_heads), int(head_dim), int(block_size), int(max_blocks))
     return SharedPrefixPlan(ext().shared_prefix_plan(group_starts, prefix_lens, seq_lens, *key), seq_lens.shape[0],
                             prefix_lens.shape[0], *key)
 
@@ -277,9 +278,9 @@ def shared_prefix_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, 
     group is shared up to that row's length.
 
     ``plan`` (:func:`shared_prefix_plan` of the same lengths) saves planning once per layer; it is
-    followed whatever the lengths are now.  Lengths and tables are device data: a table entry
-    outside the cache or group starts that descend are not followed but reported by
-    :func:`rl_b200.ops._ext.check_device_errors`.
+    followed whatever the lengths are now.  Lengths and tables are device data: table entries
+    outside the cache, lengths beyond the tables and group starts that descend are not followed but
+    reported by :func:`rl_b200.ops._ext.check_device_errors`.
     """
     _check_groups(seq_lens, group_starts, prefix_lens)
     B = q.shape[0] if q.dim() == 3 else -1
@@ -300,10 +301,9 @@ def shared_prefix_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, 
             out[live] = paged_decode_attention_ref(q[live], k_cache, v_cache, block_tables[live], seq_lens[live], scale)
         return out
     if plan is not None and plan[1:] != (B, prefix_lens.shape[0], q.shape[1], k_cache.shape[2], q.shape[2],
-                                         k_cache.shape[1]):
-        raise ValueError("shared prefix attention: a plan for (rows, groups, heads, KV heads, head dim, block size) "
-                         f"{plan[1:]} used for {B} rows, {prefix_lens.shape[0]} groups, q {tuple(q.shape)}, caches "
-                         f"{tuple(k_cache.shape)}")
+                                         k_cache.shape[1], block_tables.shape[1]):
+        raise ValueError(f"shared prefix attention: plan {plan[1:]} used for {B} rows, {prefix_lens.shape[0]} groups, "
+                         f"q {tuple(q.shape)}, caches {tuple(k_cache.shape)}, tables {tuple(block_tables.shape)}")
     if plan is None:
         add_launches(1)  # the native call plans first
     return ext().shared_prefix_attn(q, k_cache, v_cache, block_tables, seq_lens, group_starts, prefix_lens,

@@ -220,7 +220,7 @@ def test_shared_prefix_attention_repeats_and_keeps_its_inputs(cuda_device):
     b = Batch(cuda_device, [16, 8], [700, 300], [701 + i for i in range(16)] + [301 + 40 * i for i in range(8)], 32, 8,
               128, 256)
     kc, vc = b.kc.clone(), b.vc.clone()
-    plan = shared_prefix_plan(b.lens, b.starts, b.prefix, 32, 8, 128, 256)
+    plan = shared_prefix_plan(b.lens, b.starts, b.prefix, 32, 8, 128, 256, b.tables.shape[1])
     out = b.run()
     for _ in range(3):
         assert torch.equal(b.run(plan=plan), out)  # one plan for every layer, the same bits every time
@@ -231,7 +231,7 @@ def test_shared_prefix_attention_repeats_and_keeps_its_inputs(cuda_device):
 
 def test_shared_prefix_attention_refuses(cuda_device):
     b = Batch(cuda_device, [2], [64], [70, 80], 8, 2, 128, 16)
-    plan = shared_prefix_plan(b.lens, b.starts, b.prefix, 8, 2, 128, 16)
+    plan = shared_prefix_plan(b.lens, b.starts, b.prefix, 8, 2, 128, 16, b.tables.shape[1])
     with pytest.raises(ValueError):  # a plan of another batch
         b.run(plan=plan._replace(rows=3))
     with pytest.raises(RuntimeError):
@@ -266,16 +266,51 @@ def test_shared_prefix_attention_reports_bad_device_data(cuda_device):
         with pytest.raises(DeviceWaitError, match="shared_prefix"):
             check_device_errors()
     b.tables = good
-    b.lens[1] = 16 * good.shape[1] + 9  # longer than its table
-    b.run()
-    with pytest.raises(DeviceWaitError, match="shared_prefix"):
-        check_device_errors()
+    for n in (16 * good.shape[1] + 9, 2 ** 31 - 1):  # longer than its table: cut there
+        b.lens[1] = n
+        b.run()
+        with pytest.raises(DeviceWaitError, match="shared_prefix"):
+            check_device_errors()
     b.lens[1] = 80
     b.starts = torch.tensor([2, 0], dtype=torch.int32, device=cuda_device)
     b.run()
     with pytest.raises(DeviceWaitError, match="shared_prefix"):
         check_device_errors()
     b.starts = torch.tensor([0, 2], dtype=torch.int32, device=cuda_device)
+    b.check(b.run())
+
+
+def test_shared_prefix_attention_scores_out_of_range(cuda_device):
+    # a tile's first key is the reference of its scores: keys that exceed it by 2^15 and 2^60 (scores of up to
+    # thousands), a first key whose score is -inf, late keys that outgrow everything before
+    for fp8 in (False, True):
+        b = Batch(cuda_device, [3], [600], [700, 610, 1500], 8, 2, 128, 16, fp8=fp8, q_scale=8.0)
+        q = b.q[:, :1].clone()
+        b.q = q.expand(-1, 8, -1).contiguous()
+        t = b.tables.long()
+        for row, page, slot, size in ((0, 0, 0, -30.0), (0, 20, 3, 25.0), (2, 60, 1, 45.0), (2, 90, 15, 90.0)):
+            k = torch.sign(q[row, 0].float()) * size
+            k = (k / b.k_scale).clamp(-448, 448) if fp8 else k
+            b.kc[t[row, page], slot] = k.to(b.kc.dtype)
+            if page < 37:
+                for other in range(3):  # the prefix stays the same for every row
+                    b.kc[t[other, page], slot] = k.to(b.kc.dtype)
+        b.check(b.run())
+    b = Batch(cuda_device, [3], [600], [700, 610, 1500], 8, 2, 128, 16)
+    b.q = b.q.abs()
+    b.kc[b.tables[0, 0].long(), 0] = float("-inf")  # of weight 0 for every query
+    clean = b.run()
+    assert torch.isfinite(clean).all()
+    ref, tol = b.exact()
+    assert ((clean.double() - ref).abs() <= tol.nan_to_num(nan=float("inf"))).all()
+
+
+def test_shared_prefix_attention_many_rows_and_groups(cuda_device):
+    g = torch.Generator().manual_seed(3)
+    groups = torch.randint(0, 9, (150,), generator=g).tolist()
+    prefix = torch.randint(0, 400, (150,), generator=g).tolist()
+    lens = [max(1, p + int(x)) for n, p in zip(groups, prefix) for x in torch.randint(-20, 100, (n,), generator=g)]
+    b = Batch(cuda_device, groups, prefix, lens, 4, 1, 64, 16, seed=5)
     b.check(b.run())
 
 
