@@ -880,7 +880,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
 // A segment's O is stored when the group's next tile waits for the same product anyway.
 //
 // warp 0       loads K and V tiles (TMA) into a ring of entries, K and V apart
-// warp 1       issues the products, S up to two tiles ahead (of the next unit, too)
+// warp 1       issues the products, S up to three tiles ahead (of the next unit, too)
 // warp 2       brings the query rows of the next segments to shared memory
 // warps 4-11   softmax: thread r of a group owns key r of its tiles, and dim r of its output
 // warps 12-15  (e4m3 cache) convert tiles to f16, which holds e4m3 values exactly
@@ -1187,13 +1187,16 @@ __device__ __forceinline__ void refer(uint32_t t_s, int cols, float scale, float
 // a segment's outputs: thread r has dim r
 template <int HD>
 __device__ __forceinline__ void store_o(uint32_t t_o, const int* slot, float* part_o, int rn, int r) {
+
   for (int h = 0; h < rn; h += 16) {
+    int4 at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at[i] = reinterpret_cast<const int4*>(slot + h)[i];
     float o[16];
     tmem_load<16>(t_o + h, o);
-    if (r < HD)
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (h + i < rn) part_o[(long long)slot[h + i] * HD + r] = o[i];
+    for (int i = 0; i < 16; ++i)
+      if (h + i < rn && r < HD) part_o[(long long)reinterpret_cast<const int*>(at)[i] * HD + r] = o[i];
   }
 }
 
@@ -1341,12 +1344,12 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
       __syncwarp();
       if (++vi == T::VN) vi = 0, vph ^= 1;
     };
-    // whichever of the two products has its operands is issued: S up to two tiles ahead of O
+    // whichever of the two products has its operands is issued: S up to three tiles ahead of O
     int idle = 0;
     long long since = 0;
     for (int k = 0; k < ka || w.valid;) {
       bool progress = false;
-      if (w.valid && ka <= k + 2) {
+      if (w.valid && ka <= k + 3) {
         if (!q_ready) q_ready = ready(bar_q + 8 * q.bar, q.parity);
         if (q_ready && ready(bar_k + 8 * ki, kph)) {
           issue_s();
