@@ -108,17 +108,20 @@ shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __res
   // lengths are kept inside the block tables, and so short that no place on a line leaves 31 bits
   const int longest = (int)min((long long)capacity, (long long)max((1 << 30) / (nkv * units), 1) * BT);
   bool bad = false;
+  // the first of each array at once: one wait for memory instead of three
+  const int len0 = tid < B ? seq_lens[tid] : 0, share0 = tid < G ? prefix_lens[tid] : 0;
+  const int start0 = tid <= G ? group_starts[tid] : 0;
   for (int b = tid; b < B; b += kPlanThreads) {
-    const int len = max(seq_lens[b], 0);
+    const int len = max(b == tid ? len0 : seq_lens[b], 0);
     bad |= len > longest;
     s_len[b] = min(len, longest);
   }
-  for (int g = tid; g < G; g += kPlanThreads) s_share[g] = max(prefix_lens[g], 0);
+  for (int g = tid; g < G; g += kPlanThreads) s_share[g] = max(g == tid ? share0 : prefix_lens[g], 0);
   // group starts, made ascending and kept inside [0, B]: groups never overlap
   int carry = 0;
   for (int g0 = 0; g0 <= G; g0 += kPlanThreads) {
     const int g = g0 + tid;
-    const int raw = g <= G ? group_starts[g] : 0;
+    const int raw = g0 == 0 ? start0 : g <= G ? group_starts[g] : 0;
     const int v = block_scan<true>(max(carry, min(max(raw, 0), B)), s_warp);
     if (g <= G) {
       s_start[g] = v;
@@ -222,7 +225,7 @@ shared_prefix_plan_kernel(const int* __restrict__ group_starts, const int* __res
     const long long x = (long long)(suffix ? i - ctas : i) * (suffix ? per1 : per0);
     int u = 0;
     if (x < (suffix ? total1 : total0))
-      u = suffix ? nc_max + last_at_most(s_first + nc_max, B, (int)(x / nkv)) : last_at_most(s_first, nc_max, (int)(x / nkv));
+      u = suffix ? nc_max + last_at_most(s_first + nc_max, B, (int)x / nkv) : last_at_most(s_first, nc_max, (int)x / nkv);
     cta_unit[i] = u;
   }
 }
