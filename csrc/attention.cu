@@ -1019,7 +1019,7 @@ using namespace rlb;
       constexpr int HD = 16;                             \
       return __VA_ARGS__();                              \
     } else {                                             \
-      TORCH_CHECK(false, "rl_b200: head_dim ", HDV, " unsupported (16/32/64/128)"); \
+      TORCH_CHECK(false, "rl_b200: head_dim " + std::to_string(HDV) + " unsupported (16/32/64/128)"); \
     }                                                    \
   }()
 
@@ -1287,7 +1287,7 @@ at::Tensor paged_decode_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cach
     case 2: dispatch_c(std::integral_constant<int, 2>{}); break;
     case 4: dispatch_c(std::integral_constant<int, 4>{}); break;
     case 8: dispatch_c(std::integral_constant<int, 8>{}); break;
-    default: TORCH_CHECK(false, "decode: GQA group size ", G, " unsupported (1/2/4/8)");
+    default: TORCH_CHECK(false, "decode: GQA group size " + std::to_string(G) + " unsupported (1/2/4/8)");
   }
   RLB_CUDA_CHECK(cudaGetLastError());
   return out;

@@ -762,7 +762,7 @@ CUtensorMap head_tmap(const at::Tensor& x, int rows) {
   CUresult r = tma_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, x.data_ptr(), dims, strides, box, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "rl_b200 attention (tcgen05): cuTensorMapEncodeTiled failed (", (int)r, ")");
+  TORCH_CHECK(r == CUDA_SUCCESS, std::string("rl_b200 attention (tcgen05): cuTensorMapEncodeTiled failed (") + std::to_string((int)r) + ")");
   return m;
 }
 
@@ -849,7 +849,7 @@ CUtensorMap dq_tmap(const at::Tensor& x) {
   CUresult r = tma_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, x.data_ptr(), dims, strides, box, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "rl_b200 attention bwd (tcgen05): cuTensorMapEncodeTiled failed (", (int)r, ")");
+  TORCH_CHECK(r == CUDA_SUCCESS, std::string("rl_b200 attention bwd (tcgen05): cuTensorMapEncodeTiled failed (") + std::to_string((int)r) + ")");
   return m;
 }
 

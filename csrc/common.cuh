@@ -13,11 +13,15 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #define RLB_CHECK(cond, msg) TORCH_CHECK((cond), "rl_b200: ", msg)
+// Messages are made of strings only: a number formatted by a stream inside this library crashes with some
+// combinations of compiler and runtime libraries, and the process would end instead of raising.
+#define RLB_STR_(x) #x
+#define RLB_STR(x) RLB_STR_(x)
 #define RLB_CUDA_CHECK(expr)                                                      \
   do {                                                                            \
     cudaError_t _e = (expr);                                                      \
     TORCH_CHECK(_e == cudaSuccess, "rl_b200 CUDA error: ", cudaGetErrorString(_e), \
-                " at " __FILE__ ":", __LINE__);                                   \
+                " at " __FILE__ ":" RLB_STR(__LINE__));                           \
   } while (0)
 
 namespace rlb {
@@ -185,6 +189,6 @@ __device__ __forceinline__ float uniform01(uint32_t seed, uint32_t stream, uint3
       using scalar_t = float;                                               \
       return __VA_ARGS__();                                                 \
     } else {                                                                \
-      TORCH_CHECK(false, NAME, ": unsupported dtype ", (TYPE));             \
+      TORCH_CHECK(false, NAME, ": unsupported dtype ", at::toString(TYPE));             \
     }                                                                       \
   }()

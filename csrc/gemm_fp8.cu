@@ -501,7 +501,7 @@ inline CUtensorMap make_tmap_u8(const void* ptr, int64_t rows, int64_t cols, int
   CUresult r = tma_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "rl_b200: cuTensorMapEncodeTiled (u8) failed (", (int)r, ")");
+  TORCH_CHECK(r == CUDA_SUCCESS, std::string("rl_b200: cuTensorMapEncodeTiled (u8) failed (") + std::to_string((int)r) + ")");
   return m;
 }
 

@@ -504,5 +504,5 @@ void stream_write_u32(int64_t ptr, int64_t value) {
     fn = reinterpret_cast<PFN_cuStreamWriteValue32_v11070>(p);
   }
   CUresult r = fn(reinterpret_cast<CUstream>(stream()), (CUdeviceptr)ptr, (cuuint32_t)value, 0);
-  TORCH_CHECK(r == CUDA_SUCCESS, "rl_b200: cuStreamWriteValue32 failed (", (int)r, ")");
+  TORCH_CHECK(r == CUDA_SUCCESS, std::string("rl_b200: cuStreamWriteValue32 failed (") + std::to_string((int)r) + ")");
 }

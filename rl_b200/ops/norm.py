@@ -99,6 +99,8 @@ def _check_norm_fp8(x: torch.Tensor, delta, w: torch.Tensor) -> None:
     H = x.shape[-1] if x.dim() else 0
     if H == 0 or H % 128:
         raise ValueError(f"rms_norm_fp8: the hidden size must be a multiple of 128, got shape {tuple(x.shape)}")
+    if x.is_cuda and x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"rms_norm_fp8: bf16, fp16 or fp32 rows expected on a GPU, got {x.dtype}")
     if w.dim() != 1 or w.shape[0] != H or w.dtype != x.dtype or w.device != x.device:
         raise ValueError(f"rms_norm_fp8: weight {tuple(w.shape)} {w.dtype} on {w.device} for input "
                          f"{tuple(x.shape)} {x.dtype} on {x.device}")

@@ -253,6 +253,22 @@ def test_shared_prefix_attention_refuses(cuda_device):
     b.check(b.run())
 
 
+def test_refusals_with_numbers_raise(cuda_device):
+    # a number in a message of the native library
+    from rl_b200.ops.attention import paged_decode_attention
+    from rl_b200.ops.norm import rms_norm
+
+    b = Batch(cuda_device, [2], [64], [70, 80], 6, 2, 128, 16)
+    with pytest.raises(RuntimeError, match="group size 3"):
+        paged_decode_attention(b.q, b.kc, b.vc, b.tables, b.lens)
+    with pytest.raises(RuntimeError, match="head_dim 24"):
+        paged_decode_attention(b.q[:, :2, :24].contiguous(), b.kc[..., :24].contiguous(), b.vc[..., :24].contiguous(),
+                               b.tables, b.lens)
+    with pytest.raises(RuntimeError, match="unsupported dtype"), torch.no_grad():
+        rms_norm(torch.zeros(2, 64, device=cuda_device, dtype=torch.float64),
+                 torch.ones(64, device=cuda_device, dtype=torch.float64))
+
+
 def test_shared_prefix_attention_reports_bad_device_data(cuda_device):
     from rl_b200.ops._ext import DeviceWaitError, check_device_errors
 
@@ -516,6 +532,8 @@ def test_norm_fp8_special_values_views_and_empty(cuda_device):
         rms_norm_fp8(torch.zeros(2, 16512, device=cuda_device), torch.ones(16512, device=cuda_device))
     with pytest.raises(ValueError):
         rms_norm_fp8(x, w.cpu())
+    with pytest.raises(ValueError):
+        rms_norm_fp8(x.double(), w.double())
 
 
 # -------------------------------------------------------------------- the three together
