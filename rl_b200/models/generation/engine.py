@@ -128,6 +128,10 @@ class RolloutEngine:
         self._topk_steps: Optional[list] = None
         # shared prompts of the call in progress, see generate()
         self._prompts: Optional[tuple] = None
+        # decode attention over shared prompts pays from about this many cache bytes a layer saved per
+        # step (one B200, 32 / 8 heads of 128 dims): 4 MB saved, 11.3 us against 5.4 row by row;
+        # 190 MB saved, 37.5 us against 58.9
+        self.shared_prefix_min_bytes = 40 << 20
 
     # ------------------------------------------------------------ lifecycle
     def prepare_for_generation(self, num_seqs: Optional[int] = None) -> bool:
@@ -259,8 +263,12 @@ class RolloutEngine:
             for b, u in enumerate(inv):  # forked rows read their prompt's full pages where it was prefilled
                 tables[b, : lens_l[b] // bs] = tables[rep[u], : lens_l[b] // bs]
         block_tables = tables.to(dev)
-        # (prompt of every row, prompt lengths) while decode shares prompts
+        # (prompt of every row, prompt lengths) while decode attention shares prompts
         self._prompts = (torch.tensor(inv), torch.tensor([lens_l[r] for r in rep])) if share else None
+        if share and dev.type == "cuda":
+            saved = (sum(lens_l) - sum(lens_l[r] for r in rep)) * 2 * self.model.nkv * self.model.hd
+            if saved * torch.empty((), dtype=self.kv_dtype).element_size() < self.shared_prefix_min_bytes:
+                self._prompts = None  # the pages are shared all the same
         if recording:
             self.model.router_record = {}
         h_parts = []

@@ -565,6 +565,7 @@ def test_shared_prompt_rollout(cuda_device, graphs, fp8):
     from rl_b200.distributed.batched_data_dict import BatchedDataDict
     from rl_b200.models.config import ModelConfig
     from rl_b200.models.policy.worker import PolicyWorker
+    from rl_b200.parallel.state import single_process_state
 
     cfg = ModelConfig(name="small", vocab_size=2048, hidden_size=512, num_layers=3, num_heads=8, num_kv_heads=2,
                       head_dim=64, ffn_hidden_size=1408, rope_theta=10000.0, max_position_embeddings=1024)
@@ -577,9 +578,11 @@ def test_shared_prompt_rollout(cuda_device, graphs, fp8):
     if fp8:
         pcfg["generation"]["vllm_cfg"] = {"precision": "fp8", "pow2_weight_scaling_factors": True,
                                           "pow2_activation_scaling_factors": True}
-    w = PolicyWorker(pcfg, model_cfg=cfg, seed=0)
+    w = PolicyWorker(pcfg, model_cfg=cfg, pstate=single_process_state(cuda_device), seed=0)
+    assert w.engine.device.type == "cuda"
     w.engine.use_cuda_graphs = graphs
     w.engine.sync_every = 8
+    w.engine.shared_prefix_min_bytes = 0
     g = torch.Generator().manual_seed(1)
     lens = torch.tensor([200, 33, 64, 257]).repeat_interleave(4)
     ids = torch.randint(0, 2048, (4, 257), generator=g).repeat_interleave(4, 0)
@@ -596,6 +599,17 @@ def test_shared_prompt_rollout(cuda_device, graphs, fp8):
             diff = (lp - out["logprobs"])[mask].abs()
             assert mask.sum() > 16 and float(diff.mean()) < (0.1 if fp8 else 0.02)
             _ext.check_device_errors()
+            assert w.engine._prompts is not None
+        # a prompt too short to pay is forked, and attended to row by row
+        w.engine.shared_prefix_min_bytes = 1 << 40
+        out = w.generate(data)
+        assert w.engine._prompts is None
+        lp = w.get_logprobs(BatchedDataDict({"input_ids": out["output_ids"],
+                                             "input_lengths": out["unpadded_sequence_lengths"]}))["logprobs"]
+        mask = torch.zeros_like(lp, dtype=torch.bool)
+        for i in range(16):
+            mask[i, int(lens[i]): int(out["unpadded_sequence_lengths"][i])] = True
+        assert float((lp - out["logprobs"])[mask].abs().mean()) < (0.1 if fp8 else 0.02)
     finally:
         w.shutdown()
     assert w.engine.stats_last_prefill["prefilled"] == 4
