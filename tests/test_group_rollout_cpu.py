@@ -171,3 +171,24 @@ def test_rollout_without_duplicates_does_not_share():
     ref = _worker({}).generate(data, greedy=True)
     assert torch.equal(w.generate(data, greedy=True)["output_ids"], ref["output_ids"])
     assert w.engine._prompts is None
+
+
+@pytest.mark.parametrize("kv", ["auto", "fp8"])
+def test_shared_prompt_speculative_rollout(kv):
+    """Speculative decoding over forked prompts (a small LM drafts; target and draft share pages), and an
+    fp8 cache: greedy rollouts are those of copied prompts."""
+    import dataclasses
+
+    from rl_b200.models.config import get_model_config
+    from rl_b200.models.transformer import TransformerLM
+
+    outs = []
+    for mg in ({}, {"enable_shared_prefix_attention": True}):
+        w = _worker(mg)
+        w.engine.kv_dtype = torch.float8_e4m3fn if kv == "fp8" else w.engine.kv_dtype
+        draft = TransformerLM(dataclasses.replace(get_model_config("tiny-llama"), num_layers=1),
+                              device=torch.device("cpu"), dtype=torch.float32, seed=9)
+        w.engine.set_draft(draft, 3)
+        outs.append(w.generate(_batch(), greedy=True)["output_ids"])
+        assert w.engine.spec_stats["rounds"] > 0
+    assert torch.equal(outs[0], outs[1])
