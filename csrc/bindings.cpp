@@ -51,7 +51,7 @@ std::tuple<int64_t, int64_t> copy_cache_pages(at::Tensor cache, std::vector<int6
                                               std::vector<int64_t> tokens);
 // shared_prefix_attn.cu
 at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, at::Tensor seq_lens, int64_t nq,
-                              int64_t nkv, int64_t hd, int64_t block, int64_t max_blocks);
+                              int64_t nkv, int64_t hd, int64_t block, int64_t max_blocks, bool f8);
 at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor block_tables,
                               at::Tensor seq_lens, at::Tensor group_starts, at::Tensor prefix_lens,
                               c10::optional<at::Tensor> given, double scale, double k_scale, double v_scale);

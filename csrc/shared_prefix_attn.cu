@@ -19,8 +19,8 @@
 // atomics: the result does not depend on timing.
 //
 // shared_prefix_plan_kernel     group bounds, unit list, tile offsets, every CTA's first units
-// shared_prefix_tc_kernel       64 or 128 dims, pages of a multiple of 8 keys: tcgen05
-// shared_prefix_attn_kernel     everything else: mma.sync
+// shared_prefix_tc_kernel       bf16 cache, 128 dims, pages of a multiple of 8 keys: tcgen05
+// shared_prefix_attn_kernel     32, 64 and 128 dims, bf16 and e4m3, any page: mma.sync
 // shared_prefix_combine_kernel  one warp per (row, head)
 //
 // The plan depends on the lengths only: one plan serves all layers of a decode step.
@@ -48,7 +48,8 @@ struct Shape {
   int ctas, tile;
 };
 Shape shape_of(bool tc) { return tc ? Shape{num_sms(), 128} : Shape{2 * num_sms(), BT}; }
-bool use_tc(int64_t hd, int64_t block) { return (hd == 64 || hd == 128) && block % 8 == 0; }
+// The rule between the two kernels; both sides measured beside shared_prefix_attn_kernel.
+bool use_tc(int64_t hd, int64_t block, bool f8) { return hd == 128 && !f8 && block % 8 == 0; }
 
 // where the units start in a plan
 __host__ __device__ inline int unit_offset(int ctas) { return kHeader + (2 * ctas + 3) / 4 * 4; }
@@ -753,6 +754,17 @@ struct Gen {  // shared memory of the general kernel: two CTAs on an SM
 };
 
 // One producer warp and four mma.sync warps, for every head size, page size and head count.
+//
+// Bound by instructions: a 64-key tile of 64 query rows is 128 products and as many fragment loads and
+// exponentials a warp.  Against the tcgen05 kernel, kernel + plan + combine on a B200, 32 / 8 heads, in us:
+//   (prompts x rows, prompt + own keys)      this, bf16 128   tc    this, e4m3 128   tc   this, bf16 64   tc
+//   4 x 16, 1024 + 1024                             56.2   43.6             60.0   63.2            33.8  39.9
+//   8 x 16, 2048 + 1024                             88.7   74.2            100.9  126.3            55.4  61.2
+//   16 x 16, 2048 + 2048                           203.1  170.6            208.2  259.2           129.3 123.6
+//   1 x 32, 32768 + 512                            106.6   79.1            143.3  116.3            60.7  68.2
+// (tc with e4m3 converted its tiles to f16 in shared memory; with 64 dims it used half of its products' rows).
+// So bf16 caches of 128 dims go to the other kernel and the rest comes here; e4m3 needs no conversion pass, since
+// a lane's four bytes of a key are the operand words of an f16 product after one conversion each.
 template <int HD, bool F8>
 __global__ void __launch_bounds__(160, 2)
 shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -864,8 +876,8 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
 // ------------------------------------------------------------------ tcgen05 variant
 // One CTA per SM, 128 keys at a time, keys on the M side of both products:
 //
-//   S_j = K_j Q^T       M 128 keys, N query rows (16, 32 or 64), K HD
-//   O  += V_j^T P_j     M dims (twice the same 64 for HD 64), N query rows, K 128 keys
+//   S_j = K_j Q^T       M 128 keys, N query rows (16, 32 or 64), K 128 dims
+//   O  += V_j^T P_j     M 128 dims, N query rows, K 128 keys
 //
 // so that a suffix unit with a handful of query rows costs a handful of columns, and a softmax thread
 // owns a key: N exponentials per 128 keys.  Decode is bound by the cache's bytes, and this keeps the work
@@ -877,43 +889,50 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
 //
 // P = 2^(S - m) needs no maximum for its precision, only a range: m is the score of a segment's first
 // key (of the group's first tile), one per query row, so the largest P is at least 1.  bf16 has the exponents
-// of fp32, so P may reach 2^60; f16 2^15.  A barrier's OR tells when a value exceeds that; only then are
+// of fp32, so P may reach 2^60.  A barrier's OR tells when a value exceeds that; only then are
 // maxima taken (warp reductions, then across the four warps), O and the sums rescaled and P formed again.
 //
 // A segment's O is stored when the group's next tile waits for the same product anyway.
 //
-// warp 0       loads K and V tiles (TMA) into a ring of entries, K and V apart
+// warps 0, 3   load K tiles and V tiles (TMA), each into a ring of its own
 // warp 1       issues the products, S up to three tiles ahead (of the next unit, too)
 // warp 2       brings the query rows of the next segments to shared memory
 // warps 4-11   softmax: thread r of a group owns key r of its tiles, and dim r of its output
-// warps 12-15  (e4m3 cache) convert tiles to f16, which holds e4m3 values exactly
-template <int HD, bool F8>
+//
+// Measured on a B200 (kernel alone, 32 / 8 heads of 128 dims, pages of 256; the floor reads every key once at
+// the rate of a plain copy):
+//   16 prompts of up to 2048 keys x 8-16 rows with up to 2048 own keys   161 us, 5.6 TB/s (floor 139 us)
+//   4 prompts of up to 1024 keys x 8-16 rows with up to 1024 own keys     34 us, 3.6 TB/s (floor 19 us)
+//   1 prompt of 32768 keys x 32 rows                                      64 us, 2.6 TB/s (floor 26 us)
+// The first is bound by HBM.  Where prompts dominate, a tile costs about 3000 cycles of a softmax group at 64
+// columns (issue and latency of 64 exponentials a thread) against the 2770 cycles that HBM needs for its bytes
+// and half of that where two units read the same keys; short units add about a tile's time each for their
+// query rows, first scores and output.
+//
+// Tried and not kept: the two products of a query row on the M side (128 rows a unit; a suffix then costs as
+// much as a prefix), mma.sync for the suffix beside it (16-key steps are 300 instructions of latency), one
+// ring for K and V (74 against 59 us on the second case), one producer warp for both (185 against 165 us on
+// the first), issue by a plain lane 0 instead of an elected one (103 against 40 cycles a product).
 struct Tc {
-  using E = Tile<HD, false, 128>;  // K or V as the products read it (2-byte type)
-  using R = Tile<HD, F8, 128>;     // as the cache holds it
-  static constexpr int THREADS = F8 ? 512 : 384;
-  static constexpr int Q = (MR + 16) * HD * 2;  // see QPlace
+  using E = Tile<128, false, 128>;  // a K or V tile
+  static constexpr int THREADS = 384;
+  static constexpr int Q = (MR + 16) * 256;  // see QPlace
   static constexpr int P = 128 * MR * 2;
-  // places for K and V tiles as the products read them, and for raw ones.  K and V have rings of their own:
-  // a K tile is free as soon as its S is complete, a V tile only after P, and in one ring it would hold up the
-  // K tiles behind it.
-  static constexpr int KN = F8 ? (HD == 128 ? 1 : 2) : (HD == 128 ? 2 : 4);
-  static constexpr int VN = F8 ? (HD == 128 ? 2 : 3) : (HD == 128 ? 3 : 6);
-  static constexpr int RN = F8 ? (HD == 128 ? 2 : 4) : 0;  // of each
-  static constexpr int QB = 5;                     // query buffers: one for the prefix line, up to 4 for the suffix line
-  static constexpr int BARS = 2 * (KN + VN + 2 * RN) + 2 * QB + 4 + 4;
-  static constexpr int STAT = (2 + 4 + 2 + 1 + 1) * MR * 4;  // of a softmax group, see Stat
-  static constexpr int SMEM =
-      1024 + Q + 2 * P + (KN + VN) * E::BYTES + 2 * RN * R::BYTES + 2 * STAT + (MR + 16) * 4 + BARS * 8 + 16;
+  // places for K and V tiles, in rings of their own: a K tile is free as soon as its S is complete, a V tile
+  // only after P, and in one ring it would hold up the K tiles behind it
+  static constexpr int KN = 2, VN = 3;
+  static constexpr int QB = 5;  // places of query rows: one for the prefix line, up to 4 for the suffix line
+  static constexpr int BARS = 2 * (KN + VN) + 2 * QB + 4 + 4;
+  static constexpr int STAT = (2 + 4 + 2 + 1) * MR * 4;  // of a softmax group, see Stat
+  static constexpr int SMEM = 1024 + Q + 2 * P + (KN + VN) * E::BYTES + 2 * STAT + BARS * 8 + 16;
   static constexpr uint32_t COLS = 512;  // tensor memory: S four times 64, O twice 64
-  static constexpr uint32_t FMT = (1u << 4) | (8u << 24) | (F8 ? 0u : (1u << 7) | (1u << 10));  // M 128, f16 or bf16
+  static constexpr uint32_t FMT = (1u << 4) | (1u << 7) | (1u << 10) | (8u << 24);  // M 128, bf16 operands
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 // Shared-memory matrix descriptors (128-byte swizzle, 8-row groups 1024 bytes apart) in two words: the low
 // one is the address / 16, with the leading offset / 16 above it, and advances by plain additions; the high one
-// is the same for all.  The issuing thread has a few hundred cycles for the 16 products of a tile, so
-// nothing but additions is left to it.
+// is the same for all.
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t leading) { return (saddr >> 4) | ((leading >> 4) << 16); }
 template <bool ACC>
@@ -1044,21 +1063,19 @@ struct Stat {
   float* red;       // [4][MR] per warp: maxima, sums
   float* m;         // [2][MR] reference scores in use (log2)
   float* alpha;     // [MR]
-  float* c;         // [MR] score factors of the query rows (e4m3 cache)
 };
 __device__ __forceinline__ void load4(float* d, const float* s) {
   const float4 v = *reinterpret_cast<const float4*>(s);
   d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
 }
 
-template <int HD, bool F8, int N>
+template <int N>
 struct Softmax {
   static constexpr int H = N < 32 ? N : 32;  // columns at a time
-  static constexpr float kMost = F8 ? 32768.f : 1152921504606846976.f;  // 2^15, 2^60
+  static constexpr float kMost = 1152921504606846976.f;  // 2^60
 
   // 2^(S - m) of this thread's key, packed, and the largest of them
-  static __device__ __forceinline__ float weights(uint32_t* p, uint32_t t_s, bool live, float scale, const float* sm,
-                                                  const float* sc) {
+  static __device__ __forceinline__ float weights(uint32_t* p, uint32_t t_s, bool live, float scale, const float* sm) {
     float top = 0.f;
 #pragma unroll
     for (int h = 0; h < N; h += H) {
@@ -1066,18 +1083,17 @@ struct Softmax {
       tmem_load<H>(t_s + h, y);
 #pragma unroll
       for (int i = 0; i < H; i += 4) {
-        float m[4], c[4];
+        float m[4];
         load4(m, sm + h + i);
-        if (F8) load4(c, sc + h + i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          y[i + e] = ex2(y[i + e] * (F8 ? c[e] : scale) - m[e]);
+          y[i + e] = ex2(y[i + e] * scale - m[e]);
           top = fmaxf(top, y[i + e]);
         }
       }
 #pragma unroll
       for (int i = 0; i < H; i += 2) {
-        const uint32_t v = F8 ? pack_f16(y[i], y[i + 1]) : pack_bf16(y[i], y[i + 1]);
+        const uint32_t v = pack_bf16(y[i], y[i + 1]);
         p[(h + i) / 2] = live ? v : 0u;
       }
     }
@@ -1092,7 +1108,7 @@ struct Softmax {
     const int warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
 #pragma unroll 1
     for (int round = 0;; ++round) {
-      const bool over = group_any(wg, weights(p, t_s, live, scale, sm, st.c) > kMost);
+      const bool over = group_any(wg, weights(p, t_s, live, scale, sm) > kMost);
       if (!over || round > 0) break;  // after a round every value is about 1 at most
 #pragma unroll 1
       for (int h = 0; h < N; h += 16) {
@@ -1100,7 +1116,7 @@ struct Softmax {
         tmem_load<16>(t_s + h, y);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float mx = warp_max_f32(live ? y[i] * (F8 ? st.c[h + i] : scale) : -INFINITY);
+          const float mx = warp_max_f32(live ? y[i] * scale : -INFINITY);
           if (lane == i) st.red[warp4 * MR + h + i] = mx;
         }
       }
@@ -1131,8 +1147,7 @@ struct Softmax {
     }
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-      const float2 v = F8 ? __half22float2(*reinterpret_cast<__half2*>(&p[i]))
-                          : __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&p[i]));
+      const float2 v = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&p[i]));
       l[2 * i] += v.x;
       l[2 * i + 1] += v.y;
     }
@@ -1170,27 +1185,23 @@ struct Softmax {
       red[warp4 * MR + lane / (32 / N)] = l[0];
     }
   }
-
 };
 
 // the scores of a segment's first key (of the group), by the warp that has it
-template <bool F8>
-__device__ __forceinline__ void refer(uint32_t t_s, int cols, float scale, float* sm, const float* sc) {
+__device__ __forceinline__ void refer(uint32_t t_s, int cols, float scale, float* sm) {
   for (int h = 0; h < cols; h += 16) {
     float y[16];
     tmem_load<16>(t_s + h, y);
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float x = y[i] * (F8 ? sc[h + i] : scale);
+        const float x = y[i] * scale;
         sm[h + i] = x == -INFINITY ? kNoMax : x;
       }
   }
 }
 // a segment's outputs: thread r has dim r
-template <int HD>
 __device__ __forceinline__ void store_o(uint32_t t_o, const int* slot, float* part_o, int rn, int r) {
-
   for (int h = 0; h < rn; h += 16) {
     int4 at[4];
 #pragma unroll
@@ -1199,17 +1210,15 @@ __device__ __forceinline__ void store_o(uint32_t t_o, const int* slot, float* pa
     tmem_load<16>(t_o + h, o);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (h + i < rn && r < HD) part_o[(long long)reinterpret_cast<const int*>(at)[i] * HD + r] = o[i];
+      if (h + i < rn) part_o[(long long)reinterpret_cast<const int*>(at)[i] * 128 + r] = o[i];
   }
 }
 
-template <int HD, bool F8>
-__global__ void __launch_bounds__(Tc<HD, F8>::THREADS, 1)
+__global__ void __launch_bounds__(Tc::THREADS, 1)
 shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                         const __grid_constant__ Args a) {
-  using T = Tc<HD, F8>;
-  using E = typename T::E;
-  using R = typename T::R;
+  using T = Tc;
+  using E = T::E;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -1218,18 +1227,14 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
   const uint32_t s_p = s_q + T::Q;                     // [2] P of the softmax groups
   const uint32_t s_k = s_p + 2 * T::P;                 // [KN]
   const uint32_t s_v = s_k + T::KN * E::BYTES;         // [VN]
-  const uint32_t s_r = s_v + T::VN * E::BYTES;         // [2][RN] raw K, raw V
-  uint8_t* g_stat = gbase + (s_r - base) + 2 * T::RN * R::BYTES;
-  float* q_factor = reinterpret_cast<float*>(g_stat + 2 * T::STAT);  // of the rows of the query buffer
-  uint64_t* bars = reinterpret_cast<uint64_t*>(q_factor + MR + 16);
+  uint8_t* g_stat = gbase + (s_v - base) + T::VN * E::BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(g_stat + 2 * T::STAT);
   const uint32_t bar_k = smem_u32(bars);               // [KN] K ready for the products
   const uint32_t bar_kfree = bar_k + 8 * T::KN;        // [KN] K read
   const uint32_t bar_v = bar_kfree + 8 * T::KN;        // [VN] V ready
   const uint32_t bar_vfree = bar_v + 8 * T::VN;        // [VN] V read
-  const uint32_t bar_r = bar_vfree + 8 * T::VN;        // [2][RN] raw tile landed
-  const uint32_t bar_rfree = bar_r + 16 * T::RN;       // [2][RN] raw tile converted
-  const uint32_t bar_q = bar_rfree + 16 * T::RN;       // [QB] query rows ready
-  const uint32_t bar_qfree = bar_q + 8 * T::QB;        // [QB] query rows (and factors) read
+  const uint32_t bar_q = bar_vfree + 8 * T::VN;        // [QB] query rows ready
+  const uint32_t bar_qfree = bar_q + 8 * T::QB;        // [QB] query rows read
   const uint32_t bar_s = bar_qfree + 8 * T::QB;        // [4] S complete
   const uint32_t bar_p = bar_s + 32;                   // [2] S read, P written, O rescaled
   const uint32_t bar_o = bar_p + 16;                   // [2] O complete up to the tile
@@ -1242,24 +1247,18 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < T::KN; ++i) {
-      mbar_init(bar_k + 8 * i, F8 ? 4 : 1);
+      mbar_init(bar_k + 8 * i, 1);
       mbar_init(bar_kfree + 8 * i, 1);
     }
     for (int i = 0; i < T::VN; ++i) {
-      mbar_init(bar_v + 8 * i, F8 ? 4 : 1);
+      mbar_init(bar_v + 8 * i, 1);
       mbar_init(bar_vfree + 8 * i, 1);
-    }
-    for (int i = 0; i < 2 * T::RN; ++i) {
-      mbar_init(bar_r + 8 * i, 1);
-      mbar_init(bar_rfree + 8 * i, 4);
     }
     for (int i = 0; i < T::QB; ++i) {
       mbar_init(bar_q + 8 * i, 1);
-      mbar_init(bar_qfree + 8 * i, F8 ? 3 : 1);
+      mbar_init(bar_qfree + 8 * i, 1);
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(bar_s + 8 * i, 1);
-    }
+    for (int i = 0; i < 4; ++i) mbar_init(bar_s + 8 * i, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_p + 8 * i, 4);
       mbar_init(bar_o + 8 * i, 1);
@@ -1278,21 +1277,15 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
   const uint32_t tmem = *tmem_slot, t_o = tmem + 4 * MR;
   pdl_wait();
   // the walk is the same in every role: tile k belongs to softmax group k & 1
-  // (e4m3) 512 threads start with 128 registers each; the softmax groups take over what the others do not
-  // need: 2 x 80 + 2 x 168 = 496 of 4 x 128
-  if (warp < 4) {
-  if constexpr (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
   if (warp == 0 || warp == 3) {  // K tiles, V tiles
     const bool v = warp == 3;
-    const int n = F8 ? T::RN : v ? T::VN : T::KN;
-    const uint32_t full = F8 ? bar_r + 8 * v * T::RN : v ? bar_v : bar_k;
-    const uint32_t free = F8 ? bar_rfree + 8 * v * T::RN : v ? bar_vfree : bar_kfree;
-    const uint32_t dst = F8 ? s_r + v * T::RN * R::BYTES : v ? s_v : s_k;
+    const int n = v ? T::VN : T::KN;
+    const uint32_t full = v ? bar_v : bar_k, free = v ? bar_vfree : bar_kfree, dst = v ? s_v : s_k;
     Feed f;
     int k = 0, i = 0;
     uint32_t parity = 1;
     for (f.begin(a, 128); f.valid && wait(free + 8 * i, parity); ++k) {
-      f.template load<R>(a, v ? &tv : &tk, dst + i * R::BYTES, full + 8 * i);
+      f.load<E>(a, v ? &tv : &tk, dst + i * E::BYTES, full + 8 * i);
       f.next(a, 128);
       if (++i == n) i = 0, parity ^= 1;
     }
@@ -1311,13 +1304,13 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
       tc_fence_after();
       const int sb = ka & 3;
       const uint32_t n8 = columns(w.s.rn) >> 3, id = T::FMT | (n8 << 17);
-      const uint32_t kd = desc_lo(s_k + ki * E::BYTES, 0), qd = desc_lo(s_q + q.row0 * (HD * 2), 0);
+      const uint32_t kd = desc_lo(s_k + ki * E::BYTES, 0), qd = desc_lo(s_q + q.row0 * 256, 0);
       const uint32_t span = (uint32_t)q.rows * 8;  // 128 bytes a row, in units of 16
       const bool last = w.last_of_segment();
       if (elect_one()) {
         umma<false>(tmem + sb * MR, kd, qd, id, 0);
 #pragma unroll
-        for (int kk = 1; kk < HD / 16; ++kk)
+        for (int kk = 1; kk < 8; ++kk)
           umma<true>(tmem + sb * MR, kd + (kk >> 2) * 1024 + (kk & 3) * 2, qd + (kk >> 2) * span + (kk & 3) * 2, id);
         umma_commit(bar_s + 8 * sb);
         umma_commit(bar_kfree + 8 * ki);
@@ -1336,7 +1329,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
       tc_fence_after();
       const int wg = k & 1;
       const uint32_t i = info >> (8 * (k & 3)), id = T::FMT | (1u << 15) | (1u << 16) | ((i & 15u) << 17);
-      const uint32_t vd = desc_lo(s_v + vi * E::BYTES, HD == 128 ? 128 * 128 : 0), pd = desc_lo(s_p + wg * T::P, 0);
+      const uint32_t vd = desc_lo(s_v + vi * E::BYTES, 128 * 128), pd = desc_lo(s_p + wg * T::P, 0);
       if (elect_one()) {
         umma<false>(t_o + wg * MR, vd, pd, id, i & 16u);
 #pragma unroll
@@ -1377,10 +1370,9 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
         }
       }
     }
-  } else {
-    // query rows: LPR lanes a row, 16 bytes each; rows up to the segment's columns are zero
-    constexpr int LPR = HD / 8, RPI = 32 / LPR;
-    const int ch = lane % LPR, first_row = lane / LPR;
+  } else if (warp == 2) {
+    // query rows: 16 lanes a row, 16 bytes each; rows up to the segment's columns are zero
+    const int ch = lane & 15, first_row = lane >> 4;
     Walk w;
     int prefix_segs = 0;
     for (w.begin(a); w.valid;) {
@@ -1397,44 +1389,18 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
         const uint32_t rr = w.s.r0 + r, b = a.Gq == 1 ? rr : __umulhi(rr, a.inv_gq), h = rr - b * a.Gq;
         return a.q + (long long)(w.s.row0 + b) * a.q_row + (long long)(w.s.kvh * a.Gq + h) * a.q_head + ch * 8;
       };
-      const uint32_t at = q.row0 * (HD * 2) + (ch >> 3) * (q.rows * 128);
+      const uint32_t at = q.row0 * 256 + (ch >> 3) * (q.rows * 128);
       auto place = [&](int r) { return at + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
-      for (int r = first_row; r < rows; r += RPI)
+      for (int r = first_row; r < rows; r += 2)
         cp_async16_or_zero(s_q + place(r), r < w.s.rn ? src(r) : a.q, r < w.s.rn);
       asm volatile("cp.async.wait_all;\n" ::: "memory");
-      if constexpr (F8) {  // to f16, each lane the 16 bytes that it brought
-#pragma unroll 2
-        for (int r = first_row; r < rows; r += RPI) {
-          uint4 v = *reinterpret_cast<const uint4*>(gbase + place(r));
-          uint32_t* x = reinterpret_cast<uint32_t*>(&v);
-          float mx = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x[i]));
-            mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-#pragma unroll
-          for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const int ex = f16_row_exponent(mx);
-          const float f = f16_row_factor(ex);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 g = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&x[i]));
-            x[i] = pack_f16(g.x * f, g.y * f);
-          }
-          if (ch == 0) q_factor[q.row0 + r] = a.scale_log2 * f16_row_inverse(ex);
-          *reinterpret_cast<uint4*>(gbase + place(r)) = v;
-        }
-      }
       fence_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_q + 8 * q.bar);
       while (w.next(a)) {
       }
     }
-  }
-  } else if (warp < 12) {
-    if constexpr (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
+  } else {
     // every thread takes every step whatever its waits say (the error word tells): the barriers stay in step
     const int wg = (warp >> 2) - 1, r = threadIdx.x & 127;  // key of a tile, dim of the output
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16, t_og = t_o + lane_off + wg * MR;
@@ -1444,14 +1410,13 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
     st.red = reinterpret_cast<float*>(st.slot + 2 * MR);
     st.m = st.red + 4 * MR;
     st.alpha = st.m + 2 * MR;
-    st.c = st.alpha + MR;
     Walk w;
     int k = 0, mine = 0, buf = 0, left = 0;  // the group's tiles, segments mod 2, query rows whose O is not stored yet
     auto wait_o = [&] {  // the group's product before
       if (mine > 0) wait(bar_o + 8 * wg, (mine - 1) & 1);
     };
     auto flush = [&] {  // the O of the segment before
-      if (left > 0) store_o<HD>(t_og, st.slot + (buf ^ 1) * MR, a.part_o, left, r);
+      if (left > 0) store_o(t_og, st.slot + (buf ^ 1) * MR, a.part_o, left, r);
       left = 0;
     };
     for (w.begin(a); w.valid;) {
@@ -1459,11 +1424,6 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
       const bool mine0 = (k & 1) == wg;               // the segment's first tile is this group's
       const bool part = mine0 || !w.last_of_segment();  // the segment has a tile of this group
       if (part && r < s.rn) st.slot[buf * MR + r] = (int)partial_slot(a, s, w.line, mine0 ? 0 : 1, r);
-      const QPlace q(a, w.line, w.seg);
-      if (F8 && !part) {  // its factors are not read by this group
-        wait(bar_q + 8 * q.bar, q.parity);
-        if (r == 0) mbar_arrive(bar_qfree + 8 * q.bar);
-      }
       float l[MR];
 #pragma unroll
       for (int i = 0; i < MR; ++i) l[i] = 0.f;
@@ -1479,31 +1439,26 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
         tc_fence_after();
         const uint32_t t_s = tmem + lane_off + sb * MR;
         if (first) {
-          if (F8) {
-            wait(bar_q + 8 * q.bar, q.parity);
-            if (r < q.rows) st.c[r] = q_factor[q.row0 + r];
-          }
-          if ((warp & 3) == 0) refer<F8>(t_s, columns(s.rn), a.scale_log2, sm, q_factor + q.row0);
+          if ((warp & 3) == 0) refer(t_s, columns(s.rn), a.scale_log2, sm);
           group_sync(wg);
-          if (F8 && r == 0) mbar_arrive(bar_qfree + 8 * q.bar);
         }
         uint32_t p[MR / 2];
-        if (s.rn <= 16) Softmax<HD, F8, 16>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
-        else if (s.rn <= 32) Softmax<HD, F8, 32>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
-        else Softmax<HD, F8, 64>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
+        if (s.rn <= 16) Softmax<16>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
+        else if (s.rn <= 32) Softmax<32>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
+        else Softmax<64>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
         wait_o();  // it reads P's place
         tc_fence_after();
         if (first) flush();
         first = false;
-        if (s.rn <= 16) Softmax<HD, F8, 16>::write(p, prow, r);
-        else if (s.rn <= 32) Softmax<HD, F8, 32>::write(p, prow, r);
-        else Softmax<HD, F8, 64>::write(p, prow, r);
+        if (s.rn <= 16) Softmax<16>::write(p, prow, r);
+        else if (s.rn <= 32) Softmax<32>::write(p, prow, r);
+        else Softmax<64>::write(p, prow, r);
         if (nvalid < 128) {  // what lies behind the last key may be anything: P is 0 there, and V must be finite
           const int e = k % T::VN;
           wait(bar_v + 8 * e, (k / T::VN) & 1);
           if (!live)
 #pragma unroll
-            for (int i = 0; i < HD / 8; ++i)
+            for (int i = 0; i < 16; ++i)
               *reinterpret_cast<uint4*>(gbase + (s_v - base) + e * E::BYTES + E::at(r, i)) = make_uint4(0u, 0u, 0u, 0u);
         }
         fence_async();
@@ -1513,9 +1468,9 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
         ++mine;
       }
       if (part) {
-        if (s.rn <= 16) Softmax<HD, F8, 16>::reduce(l, st.red);
-        else if (s.rn <= 32) Softmax<HD, F8, 32>::reduce(l, st.red);
-        else Softmax<HD, F8, 64>::reduce(l, st.red);
+        if (s.rn <= 16) Softmax<16>::reduce(l, st.red);
+        else if (s.rn <= 32) Softmax<32>::reduce(l, st.red);
+        else Softmax<64>::reduce(l, st.red);
         group_sync(wg);
         if (r < s.rn) {
           const float m = sm[r] == kNoMax ? -INFINITY : sm[r];
@@ -1529,39 +1484,6 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
     wait_o();
     tc_fence_after();
     flush();
-  } else if constexpr (F8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
-    const int tid = threadIdx.x - 384;
-    constexpr int CH = HD / 16;  // chunks of 16 values of a key
-    Walk w;
-    int tiles = 0;
-    for (w.begin(a); w.valid; w.next(a)) ++tiles;
-    int nk = 0, nv = 0;
-    for (int e = 0; e < 2 * tiles; ++e) {
-      const bool is_k = e == 0 || ((e & 1) && nk < tiles);  // K_0, K_1, V_0, K_2, V_1, ...
-      const int c = is_k ? nk : nv, ri = c % T::RN + (is_k ? 0 : T::RN), i = is_k ? c % T::KN : c % T::VN;
-      const uint32_t full = (is_k ? bar_k : bar_v) + 8 * i, free = (is_k ? bar_kfree : bar_vfree) + 8 * i;
-      if (!wait(bar_r + 8 * ri, (c / T::RN) & 1) || !wait(free, ((is_k ? c / T::KN : c / T::VN) & 1) ^ 1)) break;
-      ++(is_k ? nk : nv);
-      const uint8_t* src = gbase + (s_r - base) + ri * R::BYTES;
-      uint8_t* dst = gbase + ((is_k ? s_k : s_v) - base) + i * E::BYTES;
-#pragma unroll 4
-      for (int x = tid; x < 128 * CH; x += 128) {
-        // 4 chunks of 8 rows a warp: the stores of a quarter warp meet no bank twice
-        const int ch = (x & 3) + 4 * (x / 512), row = (x >> 2) & 127;
-        const uint4 v = *reinterpret_cast<const uint4*>(src + R::at(row, ch));
-        *reinterpret_cast<uint4*>(dst + E::at(row, 2 * ch)) =
-            make_uint4(e4m3x2_f16x2(v.x), e4m3x2_f16x2(v.x >> 16), e4m3x2_f16x2(v.y), e4m3x2_f16x2(v.y >> 16));
-        *reinterpret_cast<uint4*>(dst + E::at(row, 2 * ch + 1)) =
-            make_uint4(e4m3x2_f16x2(v.z), e4m3x2_f16x2(v.z >> 16), e4m3x2_f16x2(v.w), e4m3x2_f16x2(v.w >> 16));
-      }
-      fence_async();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(full);
-        mbar_arrive(bar_rfree + 8 * ri);
-      }
-    }
   }
   tc_fence_before();
   __syncthreads();
@@ -1680,7 +1602,7 @@ using namespace rlb;
 // int32 plan of the work of one decode step (see the kernel): group g's rows are
 // [group_starts[g], group_starts[g+1]), of whose keys the first prefix_lens[g] are the same
 at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, at::Tensor seq_lens, int64_t nq,
-                              int64_t nkv, int64_t hd, int64_t block, int64_t max_blocks) {
+                              int64_t nkv, int64_t hd, int64_t block, int64_t max_blocks, bool f8) {
   for (at::Tensor* t : {&group_starts, &prefix_lens, &seq_lens}) {
     RLB_CHECK(t->is_cuda() && t->dim() == 1 && t->device() == seq_lens.device(),
               "shared_prefix_plan: integer vectors on one CUDA device expected");
@@ -1694,7 +1616,7 @@ at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, a
   const int capacity = (int)std::min<int64_t>(block * std::min<int64_t>(max_blocks, 1LL << 31), (1LL << 31) - 256);
   const c10::cuda::CUDAGuard guard(seq_lens.device());
   const int Gq = nq / nkv;
-  const sp::Shape p = sp::shape_of(sp::use_tc(hd, block));
+  const sp::Shape p = sp::shape_of(sp::use_tc(hd, block, f8));
   const int units = sp::max_chunks(B, G, Gq) + B;
   auto plan = at::empty({sp::plan_ints(p, units, B)}, seq_lens.options());
   const int smem = ((int)B + 4 * (int)G + 1 + units) * 4;
@@ -1733,7 +1655,7 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
     block_tables = block_tables.to(at::kInt).contiguous();
   const int64_t groups = prefix_lens.size(0);
   const int Gq = nq / nkv;
-  const bool tc = sp::use_tc(hd, bs);
+  const bool tc = sp::use_tc(hd, bs, f8);
   const sp::Shape p = sp::shape_of(tc);
   const int units = sp::max_chunks(B, groups, Gq) + B;
   for (const at::Tensor& t : {k_cache, v_cache, block_tables, seq_lens})
@@ -1745,7 +1667,7 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
   if (B == 0) return out;
   const bool planned = given.has_value() && given->defined();
   at::Tensor plan = planned ? *given : shared_prefix_plan(group_starts, prefix_lens, seq_lens, nq, nkv, hd, bs,
-                                                           block_tables.size(1));
+                                                           block_tables.size(1), f8);
   RLB_CHECK(plan.is_cuda() && plan.scalar_type() == at::kInt && plan.is_contiguous() && plan.device() == q.device() &&
                 plan.numel() == sp::plan_ints(p, units, B),
             "shared_prefix_attn: the plan is of another batch");
@@ -1784,12 +1706,11 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
   auto launch = [&](auto hdv, auto f8v) {
     constexpr int HD = decltype(hdv)::value;
     constexpr bool F8 = decltype(f8v)::value;
-    if constexpr (HD >= 64) {
+    if constexpr (HD == 128 && !F8) {
       if (tc) {
-        using T = sp::Tc<HD, F8>;
-        auto kern = sp::shared_prefix_tc_kernel<HD, F8>;
-        RLB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM));
-        sp::launch_pdl(kern, p.ctas, T::THREADS, T::SMEM, tk, tv, a);
+        auto kern = sp::shared_prefix_tc_kernel;
+        RLB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sp::Tc::SMEM));
+        sp::launch_pdl(kern, p.ctas, sp::Tc::THREADS, sp::Tc::SMEM, tk, tv, a);
       }
     }
     if (!tc) {

@@ -991,8 +991,8 @@ class TransformerLM(nn.Module):
             return lambda q, i: paged_decode_attention(q, *kv.layer(i), block_tables, seq_lens,
                                                        max_seq_len=max_seq_len, k_scale=kv.scales(i)[0],
                                                        v_scale=kv.scales(i)[1])
-        plan = (shared_prefix_plan(seq_lens, *prefix, self.nq, self.nkv, self.hd, kv.block_size, block_tables.shape[1])
-                if seq_lens.is_cuda else None)
+        plan = (shared_prefix_plan(seq_lens, *prefix, self.nq, self.nkv, self.hd, kv.block_size, block_tables.shape[1],
+                                   fp8=kv.layer(0)[0].dtype == torch.float8_e4m3fn) if seq_lens.is_cuda else None)
         return lambda q, i: shared_prefix_decode_attention(q, *kv.layer(i), block_tables, seq_lens, *prefix,
                                                            k_scale=kv.scales(i)[0], v_scale=kv.scales(i)[1], plan=plan)
 

@@ -238,6 +238,7 @@ class SharedPrefixPlan(NamedTuple):
     head_dim: int
     block_size: int
     max_blocks: int
+    fp8: bool
 
 
 def _check_groups(seq_lens, group_starts, prefix_lens):
@@ -252,14 +253,15 @@ def _check_groups(seq_lens, group_starts, prefix_lens):
 
 
 def shared_prefix_plan(seq_lens, group_starts, prefix_lens, num_heads: int, num_kv_heads: int, head_dim: int,
-                       block_size: int, max_blocks: int) -> SharedPrefixPlan:
+                       block_size: int, max_blocks: int, fp8: bool = False) -> SharedPrefixPlan:
     """Plan the attention of one decode step: which CTA takes which keys of which rows.
 
-    The plan depends on the lengths and the head, page and table sizes alone (lengths are read on
-    the device, without a synchronisation), so one plan serves every layer of the step; lengths that
-    change need a new one.  ``max_blocks`` is the width of the block tables.  GPU only."""
+    The plan depends on the lengths, the head, page and table sizes and the cache's type alone
+    (lengths are read on the device, without a synchronisation), so one plan serves every layer of
+    the step; lengths that change need a new one.  ``max_blocks`` is the width of the block tables,
+    ``fp8`` says that the cache holds e4m3.  GPU only."""
     _check_groups(seq_lens, group_starts, prefix_lens)
-    key = (int(num_heads), int(num_kv_heads), int(head_dim), int(block_size), int(max_blocks))
+    key = (int(num_heads), int(num_kv_heads), int(head_dim), int(block_size), int(max_blocks), bool(fp8))
     return SharedPrefixPlan(ext().shared_prefix_plan(group_starts, prefix_lens, seq_lens, *key), seq_lens.shape[0],
                             prefix_lens.shape[0], *key)
 
@@ -301,7 +303,8 @@ def shared_prefix_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, 
             out[live] = paged_decode_attention_ref(q[live], k_cache, v_cache, block_tables[live], seq_lens[live], scale)
         return out
     if plan is not None and plan[1:] != (B, prefix_lens.shape[0], q.shape[1], k_cache.shape[2], q.shape[2],
-                                         k_cache.shape[1], block_tables.shape[1]):
+                                         k_cache.shape[1], block_tables.shape[1],
+                                         k_cache.dtype == torch.float8_e4m3fn):
         raise ValueError(f"shared prefix attention: plan {plan[1:]} used for {B} rows, {prefix_lens.shape[0]} groups, "
                          f"q {tuple(q.shape)}, caches {tuple(k_cache.shape)}, tables {tuple(block_tables.shape)}")
     if plan is None:
