@@ -75,7 +75,7 @@ std::tuple<int64_t, int64_t> copy_cache_pages(at::Tensor cache, std::vector<int6
     if (written[src[i]]) return {4, (int64_t)i};
   if (src.empty() || cache.numel() == 0) return {none, none};
   const c10::cuda::CUDAGuard g(cache.device());
-  const long long token_bytes = cache.stride(2) * cache.element_size();
+  const long long token_bytes = cache.numel() / (planes * pages * block) * cache.element_size();
   RLB_CHECK(token_bytes < (1 << 30), "copy_cache_pages: token too large");
   const long long page_bytes = token_bytes * block, plane_bytes = page_bytes * pages;
   const bool wide = token_bytes % 16 == 0 && reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0;

@@ -1636,6 +1636,7 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
                               c10::optional<at::Tensor> given, double scale, double k_scale, double v_scale) {
   RLB_CHECK(q.is_cuda() && q.dim() == 3 && q.scalar_type() == at::kBFloat16,
             "shared_prefix_attn: q must be bf16 [rows, heads, dims]");
+  const c10::cuda::CUDAGuard guard(q.device());
   const bool f8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
   RLB_CHECK(f8 || k_cache.scalar_type() == at::kBFloat16, "shared_prefix_attn: the cache must be bf16 or e4m3");
   RLB_CHECK(k_cache.dim() == 4 && k_cache.is_contiguous() && v_cache.is_contiguous() &&
@@ -1662,7 +1663,6 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
     RLB_CHECK(t.device() == q.device(), "shared_prefix_attn: all tensors must be on one device");
   for (const at::Tensor& t : {k_cache, v_cache})
     RLB_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "shared_prefix_attn: caches must be 16-byte aligned");
-  const c10::cuda::CUDAGuard guard(q.device());
   auto out = at::empty({B, nq, hd}, q.options());
   if (B == 0) return out;
   const bool planned = given.has_value() && given->defined();

@@ -257,18 +257,16 @@ class RolloutEngine:
                                                              and not recording and ep <= 1) else 0
         rep, inv = self._unique_prompts(input_ids, lens_l) if dedup else (list(range(B)), list(range(B)))
         share = bool(mg.get("enable_shared_prefix_attention", False)) and len(rep) < B
-        if share and dev.type == "cuda" and self.model.hd not in (32, 64, 128):
-            raise ValueError(f"enable_shared_prefix_attention needs a head_dim of 32, 64 or 128, not {self.model.hd}")
+        if share and dev.type == "cuda":
+            self._check_shared_heads(spec)
         if share:
             for b, u in enumerate(inv):  # forked rows read their prompt's full pages where it was prefilled
                 tables[b, : lens_l[b] // bs] = tables[rep[u], : lens_l[b] // bs]
         block_tables = tables.to(dev)
         # (prompt of every row, prompt lengths) while decode attention shares prompts
         self._prompts = (torch.tensor(inv), torch.tensor([lens_l[r] for r in rep])) if share else None
-        if share and dev.type == "cuda":
-            saved = (sum(lens_l) - sum(lens_l[r] for r in rep)) * 2 * self.model.nkv * self.model.hd
-            if saved * torch.empty((), dtype=self.kv_dtype).element_size() < self.shared_prefix_min_bytes:
-                self._prompts = None  # the pages are shared all the same
+        if share and dev.type == "cuda" and not self._shared_prefix_pays(rep, lens_l, spec):
+            self._prompts = None  # the pages are shared all the same
         if recording:
             self.model.router_record = {}
         h_parts = []
@@ -406,6 +404,20 @@ class RolloutEngine:
         elif spec:
             self.draft.forward_prefill(flat, positions, cu_d, max(rl), self.draft_kv, slot, last_idx)
         return h
+
+    def _check_shared_heads(self, spec: bool) -> None:
+        """The heads that attention over shared prompts has kernels for, of the models that would call it."""
+        for what, m in [("model", self.model)] + ([("draft", self.draft)] if spec and self.draft_kind == "lm" else []):
+            if m.hd not in (32, 64, 128) or m.nq > 64 * m.nkv:
+                raise ValueError("enable_shared_prefix_attention needs a head_dim of 32, 64 or 128 and at most 64 query "
+                                 f"heads per KV head; the {what} has {m.nq} / {m.nkv} heads of {m.hd}")
+
+    def _shared_prefix_pays(self, rep: list[int], lens: list, spec: bool) -> bool:
+        """Whether decode attention reads each prompt once for its rows, or row by row."""
+        if len(lens) * (self.num_spec + 1 if spec else 1) > 4096:  # what a plan holds for any number of heads
+            return False
+        saved = (sum(lens) - sum(lens[r] for r in rep)) * 2 * self.model.nkv * self.model.hd
+        return saved * torch.empty((), dtype=self.kv_dtype).element_size() >= self.shared_prefix_min_bytes
 
     def _copy_prompt_blocks(self, rep: list[int], inv: list[int], lens: list, tables: torch.Tensor,
                             spec: bool) -> None:

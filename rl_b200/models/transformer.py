@@ -589,7 +589,8 @@ class TransformerLM(nn.Module):
     def _norm_lin_infer(self, x: torch.Tensor, delta: Optional[torch.Tensor], norm: str, name: str, project):
         """Rollout: RMSNorm of ``x`` (``+ delta``) and the projection ``name`` that reads it;
         returns (projection, residual stream).  With fp8 weights for ``name`` the norm quantises
-        its output itself (the same values as norm, then quantisation inside ``project``)."""
+        its output itself (the same values as norm, then quantisation inside ``project``; beyond
+        8192 values a row the two norms sum in different orders, so those keep the two steps)."""
         w, eps, fw = self._params[norm], self.cfg.rms_eps, self.fp8_weights
         if (fw is not None and self._in_rollout and self.lora is None and name in fw and x.dtype == torch.bfloat16
                 and x.shape[-1] % 128 == 0 and x.shape[-1] <= 8192):

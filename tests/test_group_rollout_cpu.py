@@ -192,3 +192,30 @@ def test_shared_prompt_speculative_rollout(kv):
         outs.append(w.generate(_batch(), greedy=True)["output_ids"])
         assert w.engine.spec_stats["rounds"] > 0
     assert torch.equal(outs[0], outs[1])
+
+
+def test_shared_prompt_rollout_rules():
+    """Which models may attend to shared prompts, and when it pays (the rules of the GPU path)."""
+    from types import SimpleNamespace as Heads
+
+    eng = _worker({"enable_shared_prefix_attention": True}).engine
+    eng.model, eng.draft, eng.draft_kind = Heads(hd=128, nq=32, nkv=8), Heads(hd=64, nq=8, nkv=2), "lm"
+    eng._check_shared_heads(True)
+    for bad in (Heads(hd=96, nq=8, nkv=8), Heads(hd=64, nq=130, nkv=2)):
+        eng.draft = bad
+        eng._check_shared_heads(False)  # the draft is not called
+        with pytest.raises(ValueError, match="draft"):
+            eng._check_shared_heads(True)
+        eng.draft_kind = "eagle3"  # attends on its own
+        eng._check_shared_heads(True)
+        eng.draft_kind, eng.model, model = "lm", bad, eng.model
+        with pytest.raises(ValueError, match="model"):
+            eng._check_shared_heads(False)
+        eng.model = model
+    # 2 x 8 x 128 values of 2 bytes a key: 10 keys saved of a prompt of 10 tokens for two rows
+    eng.kv_dtype, eng.num_spec = torch.bfloat16, 3
+    eng.shared_prefix_min_bytes = 10 * 2 * 8 * 128 * 2
+    assert eng._shared_prefix_pays([0], [10, 10], False)
+    assert not eng._shared_prefix_pays([0], [9, 9], False)
+    assert eng._shared_prefix_pays([0], [10] * 4096, False) and not eng._shared_prefix_pays([0], [10] * 4097, False)
+    assert eng._shared_prefix_pays([0], [10] * 1024, True) and not eng._shared_prefix_pays([0], [10] * 1025, True)
