@@ -151,6 +151,10 @@ rmsnorm_fwd_rowcta_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat
 // TPR = 128 is the few-row (decode) kernel, TPR = 32 the many-row one, by the same
 // rule.
 //
+// On a B200 (bf16, with delta; the norm and the quantisation as two kernels in brackets): 16384 x 4096 in
+// 93 us (237), 5.1 TB/s, bound by the latency of its loads at four blocks of 128 threads an SM, whose
+// registers hold the rows; 64 x 4096 in 2.8 us (7.3), a launch and one chain of load, sum and store.
+//
 // Scales are row-major [rows, H/128], or (mn_major) [H/128, ld] with the padding
 // rows up to ld set to 1, the layout that the hardware-scaled GEMM reads.
 template <typename T>

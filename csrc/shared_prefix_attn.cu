@@ -755,8 +755,10 @@ struct Gen {  // shared memory of the general kernel: two CTAs on an SM
 
 // One producer warp and four mma.sync warps, for every head size, page size and head count.
 //
-// Bound by instructions: a 64-key tile of 64 query rows is 128 products and as many fragment loads and
-// exponentials a warp.  Against the tcgen05 kernel, kernel + plan + combine on a B200, 32 / 8 heads, in us:
+// Bound by instructions and their latencies (e4m3: each scheduler issues 0.35 instructions a cycle for its two
+// warps; DRAM at 1.4 TB/s).  A CTA takes 3.6 us for a tile of 64 query rows with an e4m3 cache (128 products a
+// warp, and 256 conversions, which each of the four warps repeats for its own 16 rows) and 1.6 us for a tile of
+// a suffix unit, where the warps split the keys.  Against the tcgen05 kernel, kernel + plan + combine on a B200, 32 / 8 heads, in us:
 //   (prompts x rows, prompt + own keys)      this, bf16 128   tc    this, e4m3 128   tc   this, bf16 64   tc
 //   4 x 16, 1024 + 1024                             56.2   43.6             60.0   63.2            33.8  39.9
 //   8 x 16, 2048 + 1024                             88.7   74.2            100.9  126.3            55.4  61.2
@@ -1494,7 +1496,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
 
 // ----------------------------------------------------------------------- combine
 // One warp per (row, head): the partials of its prefix unit, then of its suffix unit, in the
-// order of the keys.
+// order of the keys.  Bound by latency: its launch overlaps the attention, behind which it takes 2 to 4 us.
 template <int HD>
 __global__ void __launch_bounds__(128)
 shared_prefix_combine_kernel(const int* __restrict__ plan, int ctas, int subs, int units, int B, int nq, int nkv, int Gq,

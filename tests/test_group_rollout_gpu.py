@@ -512,6 +512,32 @@ def test_norm_fp8_against_64_bits(cuda_device, dtype, rows, H):
 
 
 @torch.no_grad()
+def test_norm_fp8_equals_norm_then_quantisation_for_every_exponent(cuda_device):
+    # random mantissas and signs; x and delta of a row have exponents of a window of 16 (the first: subnormal
+    # numbers and those next to them), or of all of them, so that most sums are inexact
+    g = torch.Generator().manual_seed(3)
+    rows = 16
+    lo = torch.arange(rows)[:, None] * 16
+    lo[-1] = 0
+    width = torch.full((rows, 1), 16.0)
+    width[-1] = 250.0
+
+    def patterns():
+        e = (lo + (torch.rand(rows, 512, generator=g) * width).long()).clamp(max=250)
+        bits = (torch.randint(0, 2, e.shape, generator=g) << 15) | (e << 7) | torch.randint(0, 128, e.shape, generator=g)
+        return (bits - ((bits >> 15) << 16)).to(torch.int16).view(torch.bfloat16).to(cuda_device)
+
+    x, d = patterns(), patterns()
+    w = (1 + 0.1 * torch.randn(512, generator=g)).bfloat16().to(cuda_device)
+    for mx in (True, False):
+        for eps in (1e-5, 1e-30):
+            q, sc, s = _unfused(x, d, w, eps, mx)
+            got = add_rms_norm_fp8(x, d, w, eps, mx=mx)
+            assert torch.equal(got[2].view(torch.int16), s.view(torch.int16))
+            assert torch.equal(got[0].view(torch.uint8), q.view(torch.uint8)) and torch.equal(got[1], sc)
+
+
+@torch.no_grad()
 def test_norm_fp8_special_values_views_and_empty(cuda_device):
     w = torch.ones(256, device=cuda_device).bfloat16()
     x = torch.randn(4, 256, device=cuda_device).bfloat16()
