@@ -32,7 +32,7 @@ namespace sp {
 using namespace rlb::tc;
 typedef __nv_bfloat16 bf16;
 
-constexpr int BT = 64;        // a prefix is shared in multiples of these; keys per tile of the general kernel
+constexpr int BT = 64;        // a prefix is shared in multiples of these
 constexpr int MR = 64;        // query rows of a prefix unit
 constexpr int kMaxHeads = 64; // query heads per KV head
 constexpr int kUnitInts = 8;  // first tile, tiles, first key, keys' end, table row, first row, first query row, query rows
@@ -47,9 +47,13 @@ constexpr int kErrLengths = 1, kErrPage = 2, kErrWait = 3;  // error words
 struct Shape {
   int ctas, tile;
 };
-Shape shape_of(bool tc) { return tc ? Shape{num_sms(), 128} : Shape{2 * num_sms(), BT}; }
+// keys per tile of the general kernel; both sides measured there
+__host__ __device__ constexpr int general_tile(int hd, bool f8) { return hd <= 64 && !f8 ? 128 : 64; }
 // The rule between the two kernels; both sides measured beside shared_prefix_attn_kernel.
 bool use_tc(int64_t hd, int64_t block, bool f8) { return hd == 128 && !f8 && block % 8 == 0; }
+Shape shape_of(int64_t hd, int64_t block, bool f8) {
+  return use_tc(hd, block, f8) ? Shape{num_sms(), 128} : Shape{2 * num_sms(), general_tile((int)hd, f8)};
+}
 
 // where the units start in a plan
 __host__ __device__ inline int unit_offset(int ctas) { return kHeader + (2 * ctas + 3) / 4 * 4; }
@@ -746,7 +750,8 @@ __device__ __forceinline__ void join_warps(W& w, float* red, int stride, int wk,
 
 template <int HD, bool F8>
 struct Gen {  // shared memory of the general kernel: two CTAs on an SM
-  using C = Tile<HD, F8, BT>;
+  static constexpr int KT = general_tile(HD, F8);
+  using C = Tile<HD, F8, KT>;
   static constexpr int FIT = (112 * 1024 - kRedBytes<HD> - 1024 - 256) / (2 * C::BYTES);
   static constexpr int ST = FIT < 8 ? FIT : 8;
   static constexpr int SMEM = 1024 + ST * 2 * C::BYTES + kRedBytes<HD> + 256;
@@ -756,22 +761,37 @@ struct Gen {  // shared memory of the general kernel: two CTAs on an SM
 // One producer warp and four mma.sync warps, for every head size, page size and head count.
 //
 // Bound by instructions and their latencies (e4m3: each scheduler issues 0.35 instructions a cycle for its two
-// warps; DRAM at 1.4 TB/s).  A CTA takes 3.6 us for a tile of 64 query rows with an e4m3 cache (128 products a
-// warp, and 256 conversions, which each of the four warps repeats for its own 16 rows) and 1.6 us for a tile of
-// a suffix unit, where the warps split the keys.  Against the tcgen05 kernel, kernel + plan + combine on a B200, 32 / 8 heads, in us:
+// warps; DRAM at 1.4 TB/s).  A CTA takes 3.6 us for 64 keys x 64 query rows with an e4m3 cache of 128 dims (128
+// products a warp, and 256 conversions, which each of the four warps repeats for its own 16 rows) and 1.6 us for
+// 64 keys of a suffix unit, where the warps split the keys.
+//
+// A tile has 64 keys, or 128 for bf16 of 32 and 64 dims: longer tiles share a suffix warp's chain of products,
+// maximum and exponentials among twice the keys, but the lines are cut less evenly, and with conversions (e4m3)
+// or 128 dims there is no room in registers.  Kernel + plan + combine on a B200, 32 / 8 heads, in us, tiles of
+// 64 against 128:
+//   (prompts x rows, prompt + own keys)    bf16 32 dims    bf16 64 dims    e4m3 64 dims    e4m3 128 dims
+//   128 x 1, 1500 own keys                   48.0  40.6      62.7  54.3
+//   2 x 8, 4096 + 256                        29.5  22.6      30.0  24.3      31.1  29.2      40.4  38.5
+//   8 x 16, 2048 + 1024                      41.6  37.6      53.2  51.1      58.0  60.7     101.2 108.3
+//   16 x 16, 2048 + 2048                     80.8  71.9     111.2 111.0     120.2 126.6     207.9 218.9
+//   1 x 32, 32768 + 512                      50.2  47.9      59.8  60.7      80.7  82.0     143.7 144.5
+//
+// Against the tcgen05 kernel, the same sums:
 //   (prompts x rows, prompt + own keys)      this, bf16 128   tc    this, e4m3 128   tc   this, bf16 64   tc
-//   4 x 16, 1024 + 1024                             56.2   43.6             60.0   63.2            33.8  39.9
-//   8 x 16, 2048 + 1024                             88.7   74.2            100.9  126.3            55.4  61.2
-//   16 x 16, 2048 + 2048                           203.1  170.6            208.2  259.2           129.3 123.6
-//   1 x 32, 32768 + 512                            106.6   79.1            143.3  116.3            60.7  68.2
-// (tc with e4m3 converted its tiles to f16 in shared memory; with 64 dims it used half of its products' rows).
-// So bf16 caches of 128 dims go to the other kernel and the rest comes here; e4m3 needs no conversion pass, since
-// a lane's four bytes of a key are the operand words of an f16 product after one conversion each.
+//   4 x 16, 1024 + 1024                             56.2   43.6             59.4   63.2            32.5  39.9
+//   8 x 16, 2048 + 1024                             88.7   74.2            101.1  126.3            51.1  61.2
+//   16 x 16, 2048 + 2048                           203.1  170.6            205.4  259.2           111.0 123.6
+//   1 x 32, 32768 + 512                            106.6   79.1            142.1  116.3            60.7  68.2
+// (tc with e4m3 converted its tiles to f16 in shared memory; with 64 dims it used half of its products' rows, and
+// L2 still fetched 256 bytes a key).  So bf16 caches of 128 dims go to the other kernel and the rest comes here;
+// e4m3 needs no conversion pass, since a lane's four bytes of a key are the operand words of an f16 product
+// after one conversion each.
 template <int HD, bool F8>
 __global__ void __launch_bounds__(160, 2)
 shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                           const __grid_constant__ Args a) {
-  using C = Tile<HD, F8, BT>;
+  constexpr int KT = Gen<HD, F8>::KT;
+  using C = Tile<HD, F8, KT>;
   constexpr int ST = Gen<HD, F8>::ST;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -796,7 +816,7 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
   if (warp == 4) {
     int k = 0;
     Feed f;
-    for (f.begin(a, BT); f.valid && !*abort_flag; ++k) {
+    for (f.begin(a, KT); f.valid && !*abort_flag; ++k) {
       const int st = k % ST;
       if (!mbar_wait_err(bar_empty + 8 * st, ((k / ST) & 1) ^ 1, abort_flag, &g_shared_prefix_error, kErrWait)) break;
       const uint32_t sk = base + st * 2 * C::BYTES, sv = sk + C::BYTES;
@@ -805,8 +825,8 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
         v.template load<C>(a, &tv, sv, bar_full + 8 * st);
         f.template load<C>(a, &tk, sk, bar_full + 8 * st);
       } else {
-        const int key = f.s.k0 + f.s.j * BT;
-        for (int r = 0; r < BT; ++r) {
+        const int key = f.s.k0 + f.s.j * KT;
+        for (int r = 0; r < KT; ++r) {
           const int kr = min(key + r, f.s.k1 - 1);
           const long long slot = (long long)f.pages.get(a, f.s.trow, kr / a.block) * a.block + kr % a.block;
           const long long off = (slot * a.nkv + f.s.kvh) * C::RB;
@@ -818,13 +838,13 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
         }
         cp_async_arrive(bar_full + 8 * st);
       }
-      f.next(a, BT);
+      f.next(a, KT);
     }
     if (*abort_flag) drain(bar_full, ST, k);
     return;
   }
 
-  Warp<HD, F8, BT> w;
+  Warp<HD, F8, KT> w;
   w.lane = lane;
   w.g = lane >> 2;
   w.t = lane & 3;
@@ -836,25 +856,28 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
       // 16 query rows a warp; with fewer rows than 64 the warps split the keys instead
       const Cursor e = s;
       const int wk = e.rn <= 16 ? 4 : e.rn <= 32 ? 2 : 1;
-      const int wm = warp / wk, kq = warp % wk, key0 = kq * (BT / wk);
+      const int wm = warp / wk, kq = warp % wk, key0 = kq * (KT / wk);
       w.start(a, e, wm);
       for (bool more = true; more; ++k) {
         const int st = k % ST;
         const uint32_t sk = base + st * 2 * C::BYTES, sv = sk + C::BYTES;
-        const int nvalid = e.k1 - (e.k0 + s.j * BT);
+        const int nvalid = e.k1 - (e.k0 + s.j * KT);
         more = s.next();
         // a wait that ran out leaves the loops running on whatever is there: the error word tells
         mbar_wait_err(bar_full + 8 * st, (k / ST) & 1, abort_flag, &g_shared_prefix_error, kErrWait);
         if (wm * 16 < e.rn && key0 < nvalid) {
           if (wk == 1) {
-            if (nvalid >= BT) w.template tile<BT, false>(sk, sv, 0, BT);
-            else w.template tile<BT, true>(sk, sv, 0, nvalid);
+#pragma unroll 1
+            for (int at = 0; at < min(nvalid, KT); at += 64) {
+              if (nvalid >= at + 64) w.template tile<64, false>(sk, sv, at, KT);
+              else w.template tile<64, true>(sk, sv, at, nvalid);
+            }
           } else if (wk == 2) {
-            if (nvalid >= BT) w.template tile<BT / 2, false>(sk, sv, key0, BT);
-            else w.template tile<BT / 2, true>(sk, sv, key0, nvalid);
+            if (nvalid >= KT) w.template tile<KT / 2, false>(sk, sv, key0, KT);
+            else w.template tile<KT / 2, true>(sk, sv, key0, nvalid);
           } else {
-            if (nvalid >= BT) w.template tile<BT / 4, false>(sk, sv, key0, BT);
-            else w.template tile<BT / 4, true>(sk, sv, key0, nvalid);
+            if (nvalid >= KT) w.template tile<KT / 4, false>(sk, sv, key0, KT);
+            else w.template tile<KT / 4, true>(sk, sv, key0, nvalid);
           }
         }
         __syncwarp();
@@ -1565,9 +1588,15 @@ CUtensorMap cache_tmap(const at::Tensor& c, int box, bool f8) {
   const CUtensorMapSwizzle sw = inner == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                               : CU_TENSOR_MAP_SWIZZLE_32B;
+  // what L2 fetches at once: the bytes of a key of this head and no more, since the next head's turn comes long
+  // after (128 rows of 1500 keys of their own, 64 dims: 91 us, against 110 with 256 bytes)
+  const CUtensorMapL2promotion l2 = inner * spans >= 256  ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
+                                    : inner * spans >= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                    : inner * spans >= 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B
+                                                          : CU_TENSOR_MAP_L2_PROMOTION_NONE;
   CUresult r = tma_encode_fn()(&m, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                                c.data_ptr(), dims, strides, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                               l2, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, std::string("rl_b200: cuTensorMapEncodeTiled failed (") + std::to_string((int)r) + ")");
   return m;
 }
@@ -1618,7 +1647,7 @@ at::Tensor shared_prefix_plan(at::Tensor group_starts, at::Tensor prefix_lens, a
   const int capacity = (int)std::min<int64_t>(block * std::min<int64_t>(max_blocks, 1LL << 31), (1LL << 31) - 256);
   const c10::cuda::CUDAGuard guard(seq_lens.device());
   const int Gq = nq / nkv;
-  const sp::Shape p = sp::shape_of(sp::use_tc(hd, block, f8));
+  const sp::Shape p = sp::shape_of(hd, block, f8);
   const int units = sp::max_chunks(B, G, Gq) + B;
   auto plan = at::empty({sp::plan_ints(p, units, B)}, seq_lens.options());
   const int smem = ((int)B + 4 * (int)G + 1 + units) * 4;
@@ -1659,7 +1688,7 @@ at::Tensor shared_prefix_attn(at::Tensor q, at::Tensor k_cache, at::Tensor v_cac
   const int64_t groups = prefix_lens.size(0);
   const int Gq = nq / nkv;
   const bool tc = sp::use_tc(hd, bs, f8);
-  const sp::Shape p = sp::shape_of(tc);
+  const sp::Shape p = sp::shape_of(hd, bs, f8);
   const int units = sp::max_chunks(B, groups, Gq) + B;
   for (const at::Tensor& t : {k_cache, v_cache, block_tables, seq_lens})
     RLB_CHECK(t.device() == q.device(), "shared_prefix_attn: all tensors must be on one device");
