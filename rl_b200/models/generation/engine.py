@@ -265,7 +265,7 @@ class RolloutEngine:
         block_tables = tables.to(dev)
         # (prompt of every row, prompt lengths) while decode attention shares prompts
         self._prompts = (torch.tensor(inv), torch.tensor([lens_l[r] for r in rep])) if share else None
-        if share and dev.type == "cuda" and not self._shared_prefix_pays(rep, lens_l, spec):
+        if share and dev.type == "cuda" and not self._shared_prefix_pays(self._run_starts(inv), lens_l, spec):
             self._prompts = None  # the pages are shared all the same
         if recording:
             self.model.router_record = {}
@@ -412,11 +412,16 @@ class RolloutEngine:
                 raise ValueError("enable_shared_prefix_attention needs a head_dim of 32, 64 or 128 and at most 64 query "
                                  f"heads per KV head; the {what} has {m.nq} / {m.nkv} heads of {m.hd}")
 
-    def _shared_prefix_pays(self, rep: list[int], lens: list, spec: bool) -> bool:
-        """Whether decode attention reads each prompt once for its rows, or row by row."""
+    @staticmethod
+    def _run_starts(inv: list[int]) -> list[int]:
+        """First rows of the runs of one prompt (decode shares a prompt within a run)."""
+        return [b for b in range(len(inv)) if b == 0 or inv[b] != inv[b - 1]]
+
+    def _shared_prefix_pays(self, starts: list[int], lens: list, spec: bool) -> bool:
+        """Whether decode attention reads the prompts of the runs from ``starts`` once each, or row by row."""
         if len(lens) * (self.num_spec + 1 if spec else 1) > 4096:  # what a plan holds for any number of heads
             return False
-        saved = (sum(lens) - sum(lens[r] for r in rep)) * 2 * self.model.nkv * self.model.hd
+        saved = (sum(lens) - sum(lens[b] for b in starts)) * 2 * self.model.nkv * self.model.hd
         return saved * torch.empty((), dtype=self.kv_dtype).element_size() >= self.shared_prefix_min_bytes
 
     def _copy_prompt_blocks(self, rep: list[int], inv: list[int], lens: list, tables: torch.Tensor,

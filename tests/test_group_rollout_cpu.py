@@ -219,3 +219,12 @@ def test_shared_prompt_rollout_rules():
     assert not eng._shared_prefix_pays([0], [9, 9], False)
     assert eng._shared_prefix_pays([0], [10] * 4096, False) and not eng._shared_prefix_pays([0], [10] * 4097, False)
     assert eng._shared_prefix_pays([0], [10] * 1024, True) and not eng._shared_prefix_pays([0], [10] * 1025, True)
+
+
+def test_shared_prompt_runs():
+    """What decode saves is counted by runs: rows of one prompt that lie apart share nothing."""
+    eng = _worker({"enable_shared_prefix_attention": True}).engine
+    assert eng._run_starts([0, 0, 1, 1, 0]) == [0, 2, 4] and eng._run_starts([0, 1, 0, 1]) == [0, 1, 2, 3]
+    eng.shared_prefix_min_bytes = 1
+    assert eng._shared_prefix_pays(eng._run_starts([0, 0, 1, 1]), [9] * 4, False)
+    assert not eng._shared_prefix_pays(eng._run_starts([0, 1, 0, 1]), [9] * 4, False)
