@@ -216,6 +216,16 @@ def test_shared_prefix_attention_strided_queries_and_int64_indices(cuda_device):
     assert torch.equal(b.run(), ref)
 
 
+def test_shared_prefix_attention_of_hundreds_of_groups(cuda_device):
+    # more rows and groups than the plan takes in one pass
+    sizes = [2, 1, 3] * 100
+    prefix = [64 + 5 * (g % 40) for g in range(300)]
+    lens = [prefix[g] + (7 * r + g) % 90 for g, n in enumerate(sizes) for r in range(n)]
+    for hd, block in ((32, 16), (128, 32)):
+        b = Batch(cuda_device, sizes, prefix, lens, 4, 2, hd, block)
+        b.check(b.run())
+
+
 def test_shared_prefix_attention_repeats_and_keeps_its_inputs(cuda_device):
     b = Batch(cuda_device, [16, 8], [700, 300], [701 + i for i in range(16)] + [301 + 40 * i for i in range(8)], 32, 8,
               128, 256)
