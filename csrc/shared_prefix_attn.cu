@@ -777,7 +777,7 @@ struct Gen {  // shared memory of the general kernel: two CTAs on an SM
 // A tile has 64 keys, or 128 for bf16 of 32 and 64 dims: longer tiles share a suffix warp's chain of products,
 // maximum and exponentials among twice the keys, but the lines are cut less evenly, and with conversions (e4m3)
 // or 128 dims there is no room in registers.  Kernel + plan + combine on a B200, 32 / 8 heads, in us, tiles of
-// 64 against 128:
+// 64 against 128 (lengths are ragged, up to those stated):
 //   (prompts x rows, prompt + own keys)    bf16 32 dims    bf16 64 dims    e4m3 64 dims    e4m3 128 dims
 //   128 x 1, 1500 own keys                   48.0  40.6      62.7  54.3
 //   2 x 8, 4096 + 256                        29.5  22.6      30.0  24.3      31.1  29.2      40.4  38.5
@@ -935,9 +935,9 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
 //
 // Measured on a B200 (kernel alone, 32 / 8 heads of 128 dims, pages of 256; the floor reads every key once at
 // the rate of a plain copy):
-//   16 prompts of up to 2048 keys x 8-16 rows with up to 2048 own keys   161 us, 5.6 TB/s (floor 139 us)
+//   16 prompts of up to 2048 keys x 8-16 rows with up to 2048 own keys   160 us, 5.7 TB/s (floor 139 us)
 //   4 prompts of up to 1024 keys x 8-16 rows with up to 1024 own keys     34 us, 3.6 TB/s (floor 19 us)
-//   1 prompt of 32768 keys x 32 rows                                      64 us, 2.6 TB/s (floor 26 us)
+//   1 prompt of 32768 keys x 32 rows                                      63 us, 2.7 TB/s (floor 26 us)
 // The first is bound by HBM.  Where prompts dominate, a tile costs about 3000 cycles of a softmax group at 64
 // columns (issue and latency of 64 exponentials a thread) against the 2770 cycles that HBM needs for its bytes
 // and half of that where two units read the same keys; short units add about a tile's time each for their
