@@ -520,7 +520,7 @@ struct Warp {  // a consumer warp's state: 16 query rows, HD dims, stages of KT 
   using C = Tile<HD, F8, KT>;
   uint32_t q[HD / 16][4];
   float o[HD / 8][4];
-  float m[2], l[2], c[2];  // running maximum (log2), partial sum, score factor of rows g and g + 8
+  float m[2], l[2], c[2];  // running reference score (log2), partial sum, score factor of rows g and g + 8
   int lane, g, t;
 
   __device__ __forceinline__ void start(const Args& a, const Cursor& s, int wm) {
@@ -577,6 +577,13 @@ struct Warp {  // a consumer warp's state: 16 query rows, HD dims, stages of KT 
     for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
   }
 
+  // The score that P of a tile refers to, from the tile's largest one.  With an e4m3 cache P is an f16
+  // operand, whose values end at 2^-24: referred to the largest score, weights below 2^-25 of it would be lost
+  // (a thousand keys and more may lie there, next to one large score) though the sums count them.  Referred to
+  // 2^14 less, P reaches 2^14 (f16 ends at 2^16) and keeps its 11 bits down to 2^-28 of the largest weight.
+  // Above 2^20 the subtraction could round, past f16's end from 2^25 on; weights are 0 or 1 there anyway.
+  static __device__ __forceinline__ float reference(float mx) { return F8 && fabsf(mx) < 1048576.f ? mx - 14.f : mx; }
+
   // keys [key0, key0 + NK) of a stage of which the first nvalid are the row's
   template <int NK, bool PART>
   __device__ __forceinline__ void tile(uint32_t sk, uint32_t sv, int key0, int nvalid) {
@@ -623,7 +630,7 @@ struct Warp {  // a consumer warp's state: 16 query rows, HD dims, stages of KT 
     for (int h = 0; h < 2; ++h) {
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-      const float mn = fmaxf(m[h], mx[h]);
+      const float mn = fmaxf(m[h], reference(mx[h]));
       grew |= mn > m[h];
       mu[h] = mn == -INFINITY ? 0.f : mn;
       alpha[h] = ex2(m[h] - mu[h]);
@@ -647,7 +654,7 @@ struct Warp {  // a consumer warp's state: 16 query rows, HD dims, stages of KT 
         s[j][e] = ex2(s[j][e] - mu[e >> 1]);
         l[e >> 1] += s[j][e];
       }
-    // O += P V; P is rounded to the type of V's product (values at most 1, sums kept in fp32)
+    // O += P V; P is rounded to the type of V's product (values at most 1, or 2^14 in f16; sums kept in fp32)
 #pragma unroll
     for (int ks = 0; ks < NT / 2; ++ks) {
       uint32_t a[4];

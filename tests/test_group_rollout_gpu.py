@@ -649,3 +649,47 @@ def test_shared_prompt_rollout(cuda_device, graphs, fp8):
     finally:
         w.shutdown()
     assert w.engine.stats_last_prefill["prefilled"] == 4
+
+
+# ------------------------------------------------------- long tails, far scores, other head counts
+@pytest.mark.parametrize("binades", [20.5, 25.5, 27.5])
+@pytest.mark.parametrize("nq,nkv,hd", [(4, 4, 64), (32, 8, 128)])
+def test_shared_prefix_attention_fp8_long_tail(cuda_device, nq, nkv, hd, binades):
+    # one key of large score whose value is 0, and a thousand whose weights are 2^-binades of its: they alone make
+    # the output.  f16 weights are normal numbers down to 2^-28 of the largest (half a step: the bound's 2^-11).
+    lens = [1024 + 7 * i for i in range(40)] + [1500] * 16
+    b = Batch(cuda_device, [16], [1472], lens, nq, nkv, hd, 64, fp8=True, alone=(40, 0))
+    live = b.kc.float().isfinite()
+    b.q.fill_(1.0)
+    b.kc.copy_(torch.where(live, 0.0, b.kc.float()).to(b.kc.dtype))
+    b.vc.copy_(torch.where(live, b.vc.float().abs().clamp(min=1.0), b.vc.float()).to(b.vc.dtype))
+    first = b.tables[:, 0].long()
+    b.kc[first, 0] = torch.tensor(4.0, device=cuda_device).to(b.kc.dtype)
+    b.vc[first, 0] = torch.tensor(0.0, device=cuda_device).to(b.vc.dtype)
+    scale = binades * math.log(2) / (4.0 * b.k_scale * hd)
+    b.check(b.run(scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 19, 2.0 ** 21, 2.0 ** 25, 2.0 ** 26, 2.0 ** 40, -2.0 ** 19, -2.0 ** 26])
+def test_shared_prefix_attention_fp8_scores_of_millions(cuda_device, size):
+    # every key scores the same +-size (in powers of two), so every weight is the same number exactly: sums and the
+    # output's rounding are all that is off; then one shared key scores the opposite and is all or nothing
+    b = Batch(cuda_device, [2], [300], [310, 700], 8, 2, 128, 16, fp8=True)
+    b.q.fill_(1.0)
+    live = b.kc.float().isfinite()
+    scale = size * math.log(2) / (128 * b.k_scale)
+    b.kc.copy_(torch.where(live, 1.0, b.kc.float()).to(b.kc.dtype))
+    page, slot = int(b.tables[0, 12]), 8  # key 200
+    for opposite in (False, True):
+        if opposite:
+            b.kc[page, slot] = torch.tensor(-1.0, device=cuda_device).to(b.kc.dtype)
+        got = b.run(scale=scale)
+        for r, n in enumerate((310, 700)):
+            t = torch.arange(n, device=cuda_device)
+            slots = b.tables[r].long()[t // 16] * 16 + t % 16
+            v = b.vc.view(-1, 2, 128)[slots].double() * b.v_scale
+            if opposite:
+                v = v[200:201] if size < 0 else torch.cat([v[:200], v[201:]])
+            want = v.mean(0).repeat_interleave(4, 0)
+            tol = n * 2.0 ** -23 * v.abs().mean(0).repeat_interleave(4, 0) + 2.0 ** -8 * want.abs() + 1e-30
+            assert ((got[r].double() - want).abs() <= tol).all()
