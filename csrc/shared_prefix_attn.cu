@@ -26,6 +26,8 @@
 // The plan depends on the lengths only: one plan serves all layers of a decode step.
 #include "tc_common.cuh"
 
+#include <cfloat>
+
 namespace rlb {
 namespace sp {
 
@@ -930,7 +932,8 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
 //
 // P = 2^(S - m) needs no maximum for its precision, only a range: m is the score of a segment's first
 // key (of the group's first tile), one per query row, so the largest P is at least 1.  bf16 has the exponents
-// of fp32, so P may reach 2^60.  A barrier's OR tells when a value exceeds that; only then are
+// of fp32, so P may reach 2^60 (which leaves O room for values of V up to 2^50 over 2^17 keys).  A barrier's OR
+// tells when a value exceeds that, or a reference is so large that scores round; only then are
 // maxima taken (warp reductions, then across the four warps), O and the sums rescaled and P formed again.
 //
 // A segment's O is stored when the group's next tile waits for the same product anyway.
@@ -1096,7 +1099,10 @@ struct QPlace {
   }
 };
 
-constexpr float kNoMax = -1e30f;  // where a row has no score yet: every score exceeds it by far
+constexpr float kNoMax = -FLT_MAX;  // where a row has no score yet (-inf - -inf would be NaN): no finite score is less
+// References from this size on: score * scale - m in one rounding is off by the product's own rounding error, half a
+// binade here and any number of them far beyond (2^31: P overflows, or is 0 for the largest score itself).
+constexpr float kFar = 16777216.f;  // 2^24
 
 // what the threads of a softmax group share
 struct Stat {
@@ -1115,7 +1121,9 @@ struct Softmax {
   static constexpr int H = N < 32 ? N : 32;  // columns at a time
   static constexpr float kMost = 1152921504606846976.f;  // 2^60
 
-  // 2^(S - m) of this thread's key, packed, and the largest of them
+  // 2^(S - m) of this thread's key, packed, and the largest of them; FAR: scores are rounded as m was, so that
+  // equal ones cancel whatever their size
+  template <bool FAR>
   static __device__ __forceinline__ float weights(uint32_t* p, uint32_t t_s, bool live, float scale, const float* sm) {
     float top = 0.f;
 #pragma unroll
@@ -1128,7 +1136,7 @@ struct Softmax {
         load4(m, sm + h + i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          y[i + e] = ex2(y[i + e] * scale - m[e]);
+          y[i + e] = ex2(FAR ? __fadd_rn(__fmul_rn(y[i + e], scale), -m[e]) : y[i + e] * scale - m[e]);
           top = fmaxf(top, y[i + e]);
         }
       }
@@ -1142,22 +1150,21 @@ struct Softmax {
   }
 
   // one tile up to P (packed in p) and the sums of the rounded P in l; wait_o() waits for the group's
-  // product before
+  // product before; far: column r has a reference of kFar or more
   template <typename W>
   static __device__ __forceinline__ void tile(int wg, uint32_t t_s, uint32_t t_o, bool live, bool first, float scale,
-                                              const Stat& st, float* sm, float* l, uint32_t* p, int r, W wait_o) {
+                                              const Stat& st, float* sm, float* l, uint32_t* p, int r, bool& far,
+                                              W wait_o) {
     const int warp4 = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-#pragma unroll 1
-    for (int round = 0;; ++round) {
-      const bool over = group_any(wg, weights(p, t_s, live, scale, sm) > kMost);
-      if (!over || round > 0) break;  // after a round every value is about 1 at most
+    const float top = weights<false>(p, t_s, live, scale, sm);
+    if (group_any(wg, top > kMost || far)) {  // rare: by the maximum
 #pragma unroll 1
       for (int h = 0; h < N; h += 16) {
         float y[16];
         tmem_load<16>(t_s + h, y);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float mx = warp_max_f32(live ? y[i] * scale : -INFINITY);
+          const float mx = warp_max_f32(live ? __fmul_rn(y[i], scale) : -INFINITY);
           if (lane == i) st.red[warp4 * MR + h + i] = mx;
         }
       }
@@ -1168,6 +1175,7 @@ struct Softmax {
         const float now = fmaxf(old, mx);
         st.alpha[r] = ex2(old - now);
         sm[r] = now;
+        far = fabsf(now) >= kFar;
       }
       group_sync(wg);
       if (!first) {
@@ -1185,6 +1193,7 @@ struct Softmax {
 #pragma unroll
         for (int i = 0; i < N; ++i) l[i] *= st.alpha[i];
       }
+      weights<true>(p, t_s, live, scale, sm);  // at most 1
     }
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
@@ -1469,7 +1478,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
 #pragma unroll
       for (int i = 0; i < MR; ++i) l[i] = 0.f;
       float* sm = st.m + buf * MR;
-      bool first = true;
+      bool first = true, far = false;  // far: this thread's column has a reference of kFar or more
       for (bool same = true; same; ++k) {
         const int nvalid = s.k1 - (s.k0 + w.s.j * 128);
         same = w.next(a);
@@ -1482,11 +1491,12 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
         if (first) {
           if ((warp & 3) == 0) refer(t_s, columns(s.rn), a.scale_log2, sm);
           group_sync(wg);
+          far = r < columns(s.rn) && fabsf(sm[r]) >= kFar;
         }
         uint32_t p[MR / 2];
-        if (s.rn <= 16) Softmax<16>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
-        else if (s.rn <= 32) Softmax<32>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
-        else Softmax<64>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, wait_o);
+        if (s.rn <= 16) Softmax<16>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, far, wait_o);
+        else if (s.rn <= 32) Softmax<32>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, far, wait_o);
+        else Softmax<64>::tile(wg, t_s, t_og, live, first, a.scale_log2, st, sm, l, p, r, far, wait_o);
         wait_o();  // it reads P's place
         tc_fence_after();
         if (first) flush();
@@ -1514,8 +1524,8 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_con
         else Softmax<64>::reduce(l, st.red);
         group_sync(wg);
         if (r < s.rn) {
-          const float m = sm[r] == kNoMax ? -INFINITY : sm[r];
           const float sum = (st.red[r] + st.red[MR + r]) + (st.red[2 * MR + r] + st.red[3 * MR + r]);
+          const float m = sum == 0.f ? -INFINITY : sm[r];  // the reference counts 1 at least, unless there was no score
           *reinterpret_cast<float2*>(a.part_ml + (long long)st.slot[buf * MR + r] * 2) = make_float2(m, sum);
         }
         left = s.rn;

@@ -693,3 +693,45 @@ def test_shared_prefix_attention_fp8_scores_of_millions(cuda_device, size):
             want = v.mean(0).repeat_interleave(4, 0)
             tol = n * 2.0 ** -23 * v.abs().mean(0).repeat_interleave(4, 0) + 2.0 ** -8 * want.abs() + 1e-30
             assert ((got[r].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("size", [2.0 ** 23, 2.0 ** 26, 2.0 ** 31, 2.0 ** 40, 1e32, -2.0 ** 26, -2.0 ** 40, -1e32])
+def test_shared_prefix_attention_equal_scores_of_any_size(cuda_device, hd, size):
+    # every key scores the same, so every weight is 1 exactly, whatever the scores' size: sums, P's type and the
+    # output's rounding are all that is off; then one shared key scores the opposite and is all or nothing
+    b = Batch(cuda_device, [3], [400], [410, 700, 1500], 8, 2, hd, 16)
+    b.q.fill_(1.25)
+    live = b.kc.float().isfinite()
+    b.kc.copy_(torch.where(live, 1.0, b.kc.float()).to(b.kc.dtype))
+    page, slot = int(b.tables[0, 12]), 8  # key 200
+    for opposite in (False, True):
+        if opposite:
+            b.kc[page, slot] = -1.0
+        got = b.run(scale=size / (1.25 * hd))
+        for r, n in enumerate((410, 700, 1500)):
+            t = torch.arange(n, device=cuda_device)
+            slots = b.tables[r].long()[t // 16] * 16 + t % 16
+            v = b.vc.view(-1, 2, hd)[slots].double()
+            if opposite:
+                v = v[200:201] if size < 0 else torch.cat([v[:200], v[201:]])
+            want = v.mean(0).repeat_interleave(4, 0)
+            tol = n * 2.0 ** -23 * v.abs().mean(0).repeat_interleave(4, 0) + 2.0 ** -8 * want.abs() + 1e-30
+            assert ((got[r].double() - want).abs() <= tol).all()
+
+
+def test_shared_prefix_attention_scores_far_below_zero(cuda_device):
+    # a first key of -inf (the reference of the tiles' scores), then scores of -1e32 and less: the second key's value
+    # is the output, next to it no weight is above 0
+    for hd in (64, 128):
+        b = Batch(cuda_device, [2], [300], [310, 700], 8, 2, hd, 16)
+        b.q.fill_(1e16)
+        for r, n in enumerate([310, 700]):
+            t = torch.arange(n, device=cuda_device)
+            k = -1e14 * (1 + t.double())
+            k[0] = float("-inf")
+            slot = b.tables[r].long()[t // 16] * 16 + t % 16
+            b.kc.view(-1, 2, hd)[slot] = k.to(torch.bfloat16)[:, None, None].expand(-1, 2, hd)
+        out = b.run()
+        v = b.vc[b.tables[:, 0].long(), 1]
+        assert torch.equal(out.view(2, 2, 4, hd), v[:, :, None].expand(-1, -1, 4, -1))
