@@ -735,3 +735,21 @@ def test_shared_prefix_attention_scores_far_below_zero(cuda_device):
         out = b.run()
         v = b.vc[b.tables[:, 0].long(), 1]
         assert torch.equal(out.view(2, 2, 4, hd), v[:, :, None].expand(-1, -1, 4, -1))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_shared_prefix_attention_first_key_of_weight_zero(cuda_device, hd):
+    # as in test_shared_prefix_attention_scores_out_of_range, with the bound of the keys that count: over all of them
+    # it is infinite (the sum of |q k| is)
+    b = Batch(cuda_device, [3], [600], [700, 610, 1500], 8, 2, hd, 16)
+    b.q = b.q.abs().clamp(min=2.0 ** -6)
+    b.kc[b.tables[0, 0].long(), 0] = float("-inf")
+    got = b.run()
+    for r, n in enumerate(b.lens.tolist()):  # the row by itself behind its first key, in pages of one key
+        t = torch.arange(1, n, device=cuda_device)
+        row = object.__new__(Batch)
+        row.__dict__.update(b.__dict__, bs=1, q=b.q[r:r + 1], lens=b.lens[r:r + 1] - 1,
+                            tables=(b.tables[r].long()[t // 16] * 16 + t % 16)[None])
+        ref, tol = row.exact()
+        assert torch.isfinite(ref).all() and float(tol.max()) < 0.25
+        assert ((got[r:r + 1].double() - ref).abs() <= tol).all()
