@@ -36,10 +36,13 @@ import torch
 from rl_b200.distributed.batched_data_dict import BatchedDataDict
 from rl_b200.models.transformer import KVCache, TransformerLM
 from rl_b200.ops._ext import add_launches, launch_count
+from rl_b200.ops.attention import PAGED_DECODE_GROUPS
 from rl_b200.ops.cache_pages import copy_cache_pages
 from rl_b200.ops.sampling import sample_tokens
 
 __all__ = ["RolloutEngine"]
+
+_PLAN_ROWS = 4096  # rows that a plan of attention over shared prompts holds for any number of heads
 
 
 def _buckets(max_bs: int) -> list[int]:
@@ -256,16 +259,23 @@ class RolloutEngine:
         chunk_tokens = int(mg.get("max_tokens", 16384)) if (mg.get("enable_chunked_prefill", True)
                                                              and not recording and ep <= 1) else 0
         rep, inv = self._unique_prompts(input_ids, lens_l) if dedup else (list(range(B)), list(range(B)))
-        share = bool(mg.get("enable_shared_prefix_attention", False)) and len(rep) < B
-        if share and dev.type == "cuda":
+        enabled = bool(mg.get("enable_shared_prefix_attention", False))
+        share = enabled and len(rep) < B
+        # heads that row-by-row attention lacks: every batch attends by prompts, whatever that saves
+        only = enabled and dev.type == "cuda" and not self._row_by_row_heads(spec)
+        if (share or only) and dev.type == "cuda":
             self._check_shared_heads(spec)
+        if only and not self._fits_plan(B, spec):
+            raise ValueError(f"{B} sequences are too many for a model whose query heads per KV head are none of "
+                             f"{PAGED_DECODE_GROUPS}: attention over shared prompts takes {_PLAN_ROWS} rows a step"
+                             + (f", here {self.num_spec + 1} a sequence" if spec else ""))
         if share:
             for b, u in enumerate(inv):  # forked rows read their prompt's full pages where it was prefilled
                 tables[b, : lens_l[b] // bs] = tables[rep[u], : lens_l[b] // bs]
         block_tables = tables.to(dev)
         # (prompt of every row, prompt lengths) while decode attention shares prompts
-        self._prompts = (torch.tensor(inv), torch.tensor([lens_l[r] for r in rep])) if share else None
-        if share and dev.type == "cuda" and not self._shared_prefix_pays(self._run_starts(inv), lens_l, spec):
+        self._prompts = (torch.tensor(inv), torch.tensor([lens_l[r] for r in rep])) if share or only else None
+        if share and not only and dev.type == "cuda" and not self._shared_prefix_pays(self._run_starts(inv), lens_l, spec):
             self._prompts = None  # the pages are shared all the same
         if recording:
             self.model.router_record = {}
@@ -405,9 +415,20 @@ class RolloutEngine:
             self.draft.forward_prefill(flat, positions, cu_d, max(rl), self.draft_kv, slot, last_idx)
         return h
 
+    def _attending(self, spec: bool) -> list[tuple]:
+        """The models whose decode attention the engine chooses."""
+        return [("model", self.model)] + ([("draft", self.draft)] if spec and self.draft_kind == "lm" else [])
+
+    def _row_by_row_heads(self, spec: bool) -> bool:
+        """Whether the kernel that attends row by row takes the heads of every such model."""
+        return all(m.nq // m.nkv in PAGED_DECODE_GROUPS for _, m in self._attending(spec))
+
+    def _fits_plan(self, sequences: int, spec: bool) -> bool:
+        return sequences * (self.num_spec + 1 if spec else 1) <= _PLAN_ROWS
+
     def _check_shared_heads(self, spec: bool) -> None:
-        """The heads that attention over shared prompts has kernels for, of the models that would call it."""
-        for what, m in [("model", self.model)] + ([("draft", self.draft)] if spec and self.draft_kind == "lm" else []):
+        """The heads that attention over shared prompts has kernels for."""
+        for what, m in self._attending(spec):
             if m.hd not in (32, 64, 128) or m.nq > 64 * m.nkv:
                 raise ValueError("enable_shared_prefix_attention needs a head_dim of 32, 64 or 128 and at most 64 query "
                                  f"heads per KV head; the {what} has {m.nq} / {m.nkv} heads of {m.hd}")
@@ -419,7 +440,7 @@ class RolloutEngine:
 
     def _shared_prefix_pays(self, starts: list[int], lens: list, spec: bool) -> bool:
         """Whether decode attention reads the prompts of the runs from ``starts`` once each, or row by row."""
-        if len(lens) * (self.num_spec + 1 if spec else 1) > 4096:  # what a plan holds for any number of heads
+        if not self._fits_plan(len(lens), spec):
             return False
         saved = (sum(lens) - sum(lens[b] for b in starts)) * 2 * self.model.nkv * self.model.hd
         return saved * torch.empty((), dtype=self.kv_dtype).element_size() >= self.shared_prefix_min_bytes

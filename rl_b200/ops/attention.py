@@ -32,6 +32,7 @@ from rl_b200.ops._ext import add_launches, ext, use_native
 __all__ = [
     "flash_attn_varlen",
     "flash_attn_varlen_ref",
+    "PAGED_DECODE_GROUPS",
     "paged_decode_attention",
     "paged_decode_attention_ref",
     "SharedPrefixPlan",
@@ -210,6 +211,10 @@ def paged_decode_attention_ref(q, k_cache, v_cache, block_tables, seq_lens, scal
         sc = torch.einsum("hd,hld->hl", q[b].float(), kb) * scale
         out[b] = torch.einsum("hl,hld->hd", torch.softmax(sc, -1), vb)
     return out.to(q.dtype)
+
+
+# query heads per KV head that the kernel of paged_decode_attention has (csrc/attention.cu)
+PAGED_DECODE_GROUPS = (1, 2, 4, 8)
 
 
 def paged_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, scale: Optional[float] = None,

@@ -228,3 +228,20 @@ def test_shared_prompt_runs():
     eng.shared_prefix_min_bytes = 1
     assert eng._shared_prefix_pays(eng._run_starts([0, 0, 1, 1]), [9] * 4, False)
     assert not eng._shared_prefix_pays(eng._run_starts([0, 1, 0, 1]), [9] * 4, False)
+
+
+def test_heads_that_row_by_row_attention_lacks():
+    """Query heads per KV head decide whether attention by prompts is a choice (the rule of the GPU path)."""
+    from types import SimpleNamespace as Heads
+
+    eng = _worker({"enable_shared_prefix_attention": True}).engine
+    eng.draft, eng.draft_kind, eng.num_spec = Heads(hd=128, nq=8, nkv=1), "lm", 3
+    for nq, nkv, row_by_row in ((32, 8, True), (8, 8, True), (64, 8, True), (28, 4, False), (12, 2, False), (5, 1, False)):
+        eng.model = Heads(hd=128, nq=nq, nkv=nkv)
+        assert eng._row_by_row_heads(False) == eng._row_by_row_heads(True) == row_by_row
+    eng.model, eng.draft = Heads(hd=128, nq=8, nkv=1), Heads(hd=128, nq=28, nkv=4)
+    assert eng._row_by_row_heads(False) and not eng._row_by_row_heads(True)
+    eng.draft_kind = "eagle3"  # attends on its own
+    assert eng._row_by_row_heads(True)
+    assert eng._fits_plan(4096, False) and not eng._fits_plan(4097, False)
+    assert eng._fits_plan(1024, True) and not eng._fits_plan(1025, True)

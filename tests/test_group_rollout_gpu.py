@@ -753,3 +753,70 @@ def test_shared_prefix_attention_first_key_of_weight_zero(cuda_device, hd):
         ref, tol = row.exact()
         assert torch.isfinite(ref).all() and float(tol.max()) < 0.25
         assert ((got[r:r + 1].double() - ref).abs() <= tol).all()
+
+
+def _rollout_worker(dev, heads, kv_heads, head_dim, vocab=2048, stop=(), vllm=None, layers=2):
+    from rl_b200.models.config import ModelConfig
+    from rl_b200.models.policy.worker import PolicyWorker
+    from rl_b200.parallel.state import single_process_state
+
+    cfg = ModelConfig(name="small", vocab_size=vocab, hidden_size=512, num_layers=layers, num_heads=heads,
+                      num_kv_heads=kv_heads, head_dim=head_dim, ffn_hidden_size=1408, rope_theta=10000.0,
+                      max_position_embeddings=1024)
+    pcfg = {"model_name": "small", "max_total_sequence_length": 320, "precision": "bfloat16",
+            "train_global_batch_size": 16, "train_micro_batch_size": 4,
+            "generation": {"temperature": 1.0, "top_p": 1.0, "top_k": None, "max_new_tokens": 40,
+                           "stop_token_ids": list(stop), "vllm_cfg": vllm or {},
+                           "mcore_generation_config": {"block_size_tokens": 16,
+                                                       "enable_shared_prefix_attention": True}},
+            "sequence_packing": {"train_mb_tokens": 2048, "logprob_mb_tokens": 2048}}
+    return PolicyWorker(pcfg, model_cfg=cfg, pstate=single_process_state(dev), seed=0), cfg
+
+
+def _rollout_batch(copies, vocab=2048):
+    from rl_b200.distributed.batched_data_dict import BatchedDataDict
+
+    g = torch.Generator().manual_seed(1)
+    n = 16 // copies
+    lens = torch.tensor(([200, 33, 64, 257] * 4)[:n]).repeat_interleave(copies)
+    ids = torch.randint(0, vocab, (n, 257), generator=g).repeat_interleave(copies, 0)
+    return BatchedDataDict({"input_ids": ids, "input_lengths": lens})
+
+
+def _logprob_gap(w, data, out):
+    from rl_b200.distributed.batched_data_dict import BatchedDataDict
+
+    lp = w.get_logprobs(BatchedDataDict({"input_ids": out["output_ids"],
+                                         "input_lengths": out["unpadded_sequence_lengths"]}))["logprobs"]
+    mask = torch.zeros_like(lp, dtype=torch.bool)
+    for i, n in enumerate(data["input_lengths"].tolist()):
+        mask[i, n: int(out["unpadded_sequence_lengths"][i])] = True
+    return float((lp - out["logprobs"])[mask].abs().mean())
+
+
+@pytest.mark.parametrize("spec", [False, True])
+@pytest.mark.parametrize("kv", ["auto", "fp8"])
+@pytest.mark.parametrize("copies", [4, 1])
+@pytest.mark.parametrize("heads,head_dim", [(14, 128), (6, 64)])
+def test_rollout_of_heads_that_only_shared_prompts_take(cuda_device, heads, head_dim, copies, kv, spec, monkeypatch):
+    # query heads per KV head that row-by-row attention lacks: prompts too short to pay, with copies and without
+    import dataclasses
+
+    from rl_b200.models.transformer import TransformerLM
+
+    w, cfg = _rollout_worker(cuda_device, heads, 2, head_dim, vllm={"kv_cache_dtype": kv})
+    w.engine.sync_every = 8
+    if spec:
+        w.engine.set_draft(TransformerLM(dataclasses.replace(cfg, num_layers=1), device=cuda_device,
+                                         dtype=torch.bfloat16, seed=9), 3)
+    data = _rollout_batch(copies)
+    try:
+        out = w.generate(data)
+        assert _logprob_gap(w, data, out) < (0.1 if kv == "fp8" else 0.02)
+        _ext.check_device_errors()
+        if heads == 6 and copies == 1:  # more rows than a plan takes: refused before the prefill
+            monkeypatch.setattr("rl_b200.models.generation.engine._PLAN_ROWS", 63 if spec else 15)
+            with pytest.raises(ValueError, match="16 sequences"):
+                w.generate(data)
+    finally:
+        w.shutdown()
