@@ -68,6 +68,7 @@ class _DecodeState:
         # rows that share a prompt: their bounds and the prompt's length (unused groups are empty)
         self.group_starts = torch.zeros(B + 1, dtype=i32, device=device)
         self.prefix_lens = torch.zeros(B, dtype=i32, device=device)
+        self.shares = False
         self.done = torch.ones(B, dtype=torch.bool, device=device)
         self.gen_len = torch.zeros(B, dtype=i32, device=device)
         self.max_new = torch.zeros(B, dtype=i32, device=device)
@@ -131,6 +132,7 @@ class RolloutEngine:
         self._topk_steps: Optional[list] = None
         # shared prompts of the call in progress, see generate()
         self._prompts: Optional[tuple] = None
+        self._only_by_prompts = False
         # decode attention over shared prompts pays from about this many cache bytes a layer saved per
         # step (one B200, 32 / 8 heads of 128 dims): 4 MB saved, 11.3 us against 5.4 row by row;
         # 190 MB saved, 37.5 us against 58.9
@@ -262,7 +264,7 @@ class RolloutEngine:
         enabled = bool(mg.get("enable_shared_prefix_attention", False))
         share = enabled and len(rep) < B
         # heads that row-by-row attention lacks: every batch attends by prompts, whatever that saves
-        only = enabled and dev.type == "cuda" and not self._row_by_row_heads(spec)
+        self._only_by_prompts = only = enabled and dev.type == "cuda" and not self._row_by_row_heads(spec)
         if (share or only) and dev.type == "cuda":
             self._check_shared_heads(spec)
         if only and not self._fits_plan(B, spec):
@@ -444,6 +446,15 @@ class RolloutEngine:
             return False
         saved = (sum(lens) - sum(lens[b] for b in starts)) * 2 * self.model.nkv * self.model.hd
         return saved * torch.empty((), dtype=self.kv_dtype).element_size() >= self.shared_prefix_min_bytes
+
+    def _shares_prompts(self, rows: torch.Tensor) -> bool:
+        """Whether decode attention of the rows that are left goes by prompts: what pays for the whole batch
+        need not pay for its last rows."""
+        if self._prompts is None or self._only_by_prompts:
+            return self._prompts is not None
+        prompt, lens = self._prompts
+        p = prompt[rows.cpu()]
+        return self._shared_prefix_pays(self._run_starts(p.tolist()), lens[p].tolist(), False)
 
     def _copy_prompt_blocks(self, rep: list[int], inv: list[int], lens: list, tables: torch.Tensor,
                             spec: bool) -> None:
@@ -667,7 +678,7 @@ class RolloutEngine:
         while rows.numel() > 0 and step_done < max_new:
             nb = next(b for b in _buckets(self.max_num_seqs) if b >= rows.numel()) \
                 if rows.numel() <= self.max_num_seqs else rows.numel()
-            st = self._state(nb, max_new, (temperature, top_k, top_p, self._prompts is not None))
+            st = self._state(nb, max_new, (temperature, top_k, top_p, self._shares_prompts(rows)))
             n = rows.numel()
             st.stop.fill_(-1)
             st.stop[: min(len(stop_ids), st.stop.numel())] = stop[: st.stop.numel()] if stop_ids else -1
@@ -679,7 +690,7 @@ class RolloutEngine:
             st.positions[:n] = (lengths[rows] + step_done - 1).to(torch.int32)
             st.block_tables.zero_()
             st.block_tables[:n] = block_tables[rows]
-            if self._prompts is not None:
+            if st.shares:
                 self._prefix_groups(rows, out=(st.group_starts, st.prefix_lens))
             st.gen_len.zero_()
             st.gen_len[:n] = glen[rows]
@@ -719,12 +730,14 @@ class RolloutEngine:
         return tokens_all, lps_all, glen
 
     def _state(self, nb: int, max_new: int, sampling_key: tuple = ()) -> _DecodeState:
-        """Decode buffers + graph for one batch bucket.  Sampling parameters are
-        baked into a captured graph, so they are part of the cache key."""
+        """Decode buffers + graph for one batch bucket.  Sampling parameters, and whether decode
+        attention goes by prompts (the last of them), are baked into a captured graph, so they are part of
+        the cache key."""
         key = (nb,) + tuple(sampling_key)
         st = self._states.get(key)
         if st is None or st.out_tokens.shape[1] < max_new + 1:
             st = _DecodeState(nb, self.max_blocks_per_seq, max_new, self.device)
+            st.shares = bool(sampling_key and sampling_key[-1])
             self._states[key] = st
         return st
 
@@ -736,7 +749,7 @@ class RolloutEngine:
         st.seq_lens.copy_(st.positions + 1)
         h = self.model.forward_decode(st.tokens, st.positions, self.kv, st.block_tables, st.seq_lens, st.slot,
                                       self.max_model_len,
-                                      prefix=(st.group_starts, st.prefix_lens) if self._prompts is not None else None)
+                                      prefix=(st.group_starts, st.prefix_lens) if st.shares else None)
         logits = self.model.logits_infer(h)
         from rl_b200.ops.sampling import sample_tokens_graphable
 

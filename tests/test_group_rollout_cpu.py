@@ -245,3 +245,16 @@ def test_heads_that_row_by_row_attention_lacks():
     assert eng._row_by_row_heads(True)
     assert eng._fits_plan(4096, False) and not eng._fits_plan(4097, False)
     assert eng._fits_plan(1024, True) and not eng._fits_plan(1025, True)
+
+
+def test_rows_that_are_left_share_where_it_pays_for_them():
+    eng = _worker({"enable_shared_prefix_attention": True}).engine
+    assert not eng._shares_prompts(torch.arange(4))  # no shared prompts
+    eng._prompts = (torch.tensor([0, 0, 0, 1, 1, 2, 0]), torch.tensor([10, 20, 30]))
+    token = 2 * eng.model.nkv * eng.model.hd * torch.empty((), dtype=eng.kv_dtype).element_size()
+    for limit, rows, shares in ((40, range(7), True), (41, range(7), False), (20, [0, 1, 2], True), (21, [0, 1, 2], False),
+                                (20, [2, 3, 4], True), (1, [0, 3, 5, 6], False), (10, [0, 1, 5], True), (1, [2], False)):
+        eng.shared_prefix_min_bytes = limit * token
+        assert eng._shares_prompts(torch.tensor(list(rows))) == shares
+    eng._only_by_prompts = True
+    assert eng._shares_prompts(torch.tensor([2]))

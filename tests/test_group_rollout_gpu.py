@@ -820,3 +820,23 @@ def test_rollout_of_heads_that_only_shared_prompts_take(cuda_device, heads, head
                 w.generate(data)
     finally:
         w.shutdown()
+
+
+@pytest.mark.parametrize("heads", [8, 6])
+def test_rollout_decides_again_for_the_rows_that_are_left(cuda_device, heads):
+    # 16 rows save 851 kB a layer, the 8 rows or fewer of the next batch 702 kB at most (4 of 257 and 4 of 200 tokens)
+    w, _ = _rollout_worker(cuda_device, heads, 2, 64, vocab=256, stop=range(8))
+    w.engine.sync_every = 8
+    w.engine.shared_prefix_min_bytes = 750_000
+    seen, state = [], w.engine._state
+    w.engine._state = lambda nb, max_new, key: (seen.append((nb, key[-1])), state(nb, max_new, key))[1]
+    data = _rollout_batch(4, 256)
+    try:
+        out = w.generate(data)
+        assert seen[0] == (16, True) and len(seen) > 1 and seen[1][0] <= 8
+        # 3 query heads per KV head have no other way
+        assert all(shares == (heads == 6) for _, shares in seen[1:])
+        assert _logprob_gap(w, data, out) < 0.02
+        _ext.check_device_errors()
+    finally:
+        w.shutdown()
