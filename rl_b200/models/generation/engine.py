@@ -133,10 +133,9 @@ class RolloutEngine:
         # shared prompts of the call in progress, see generate()
         self._prompts: Optional[tuple] = None
         self._only_by_prompts = False
-        # decode attention over shared prompts pays from about this many cache bytes a layer saved per
-        # step (one B200, 32 / 8 heads of 128 dims): 4 MB saved, 11.3 us against 5.4 row by row;
-        # 190 MB saved, 37.5 us against 58.9
-        self.shared_prefix_min_bytes = 40 << 20
+        # cache bytes a layer that decode attention by prompts must save per step (None: what pays, by
+        # _shared_prefix_limit)
+        self.shared_prefix_min_bytes: Optional[int] = None
 
     # ------------------------------------------------------------ lifecycle
     def prepare_for_generation(self, num_seqs: Optional[int] = None) -> bool:
@@ -444,8 +443,28 @@ class RolloutEngine:
         """Whether decode attention reads the prompts of the runs from ``starts`` once each, or row by row."""
         if not self._fits_plan(len(lens), spec):
             return False
-        saved = (sum(lens) - sum(lens[b] for b in starts)) * 2 * self.model.nkv * self.model.hd
-        return saved * torch.empty((), dtype=self.kv_dtype).element_size() >= self.shared_prefix_min_bytes
+        size = torch.empty((), dtype=self.kv_dtype).element_size()
+        saved = (sum(lens) - sum(lens[b] for b in starts)) * 2 * self.model.nkv * self.model.hd * size
+        limit = self.shared_prefix_min_bytes
+        return saved >= (self._shared_prefix_limit(len(lens), size) if limit is None else limit)
+
+    def _shared_prefix_limit(self, rows: int, size: int) -> int:
+        """Bytes saved a layer from which attention by prompts is the faster one, for a cache of ``size`` bytes a
+        value.  Measured on a B200 (us a layer, its share of the plan included, against row by row) with 1 to 64
+        prompts x 4 to 64 rows, 1 to 8 query heads on 2, 4 and 8 KV heads and up to 32, 512 and 2048 own tokens a
+        row; the figures are for 32 / 8 heads and 32 own tokens:
+
+        * bf16, 128 dims: 16 rows 16.7 against 12.4 with 40 MB saved, 20.9 / 18.7 with 80, 26.8 / 30.9 with 160; 64
+          rows 20.7 / 16.9, 23.0 / 19.0 and 23.2 / 40.6; 256 rows 29.7 / 29.5, 39.5 / 39.2 and 39.5 / 48.1.  From
+          100 MB on the ratio is 1.10 at worst and 0.56 at best; with 40 to 80 MB it is between 1.72 and 0.72.
+        * bf16, 64 dims, where a row's own part costs more: 16 rows 17.7 / 11.9 with 40 MB, 25.7 / 32.3 with 160; 256
+          rows 31.3 / 27.6 with 160 MB, 35.5 / 46.0 with 320; 1024 rows 108 / 87 with 480.  From 80 MB and 96 kB for
+          every row and KV head on 1.04 and 0.41; below, up to 2.8.
+        * e4m3, and 32 dims, which row by row attends to without tensor cores: from 40 MB on 0.41 and 0.09."""
+        m = self.model
+        if size == 1 or m.hd == 32:
+            return 40 << 20
+        return 100 << 20 if m.hd == 128 else (80 << 20) + rows * m.nkv * (96 << 10)
 
     def _shares_prompts(self, rows: torch.Tensor) -> bool:
         """Whether decode attention of the rows that are left goes by prompts: what pays for the whole batch

@@ -258,3 +258,18 @@ def test_rows_that_are_left_share_where_it_pays_for_them():
         assert eng._shares_prompts(torch.tensor(list(rows))) == shares
     eng._only_by_prompts = True
     assert eng._shares_prompts(torch.tensor([2]))
+
+
+@pytest.mark.parametrize("dtype,hd,nkv,rows,limit", [
+    (torch.bfloat16, 128, 8, 16, 100 << 20), (torch.bfloat16, 64, 8, 256, 272 << 20), (torch.bfloat16, 64, 2, 16, 83 << 20),
+    (torch.float8_e4m3fn, 128, 8, 16, 40 << 20), (torch.float8_e4m3fn, 64, 8, 256, 40 << 20),
+    (torch.bfloat16, 32, 8, 64, 40 << 20)])
+def test_shared_prompts_pay_by_type_heads_and_rows(dtype, hd, nkv, rows, limit):
+    from types import SimpleNamespace as Heads
+
+    eng = _worker({"enable_shared_prefix_attention": True}).engine
+    eng.model, eng.kv_dtype = Heads(hd=hd, nq=4 * nkv, nkv=nkv), dtype
+    token = 2 * nkv * hd * dtype.itemsize
+    tokens = -(-limit // (token * (rows - 1)))  # of one prompt for all the rows
+    assert eng._shared_prefix_pays([0], [tokens] * rows, False)
+    assert not eng._shared_prefix_pays([0], [tokens - 1] * rows, False)
