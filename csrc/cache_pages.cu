@@ -53,8 +53,8 @@ copy_pages_kernel(const __grid_constant__ Pairs p, int n, uint8_t* __restrict__ 
 
 using namespace rlb;
 
-// cache [planes, pages, block, ...] contiguous, updated in place.  Returns (0, 0), or what is wrong
-// with the page lists and at which pair (nothing is copied then): 1 a page outside the cache,
+// cache [planes, pages, block, ...] contiguous, updated in place.  Returns (0, kernels launched), or what is
+// wrong with the page lists and at which pair (nothing is copied then): 1 a page outside the cache,
 // 2 a token count outside the page, 3 a page written twice, 4 a page both read and written.
 std::tuple<int64_t, int64_t> copy_cache_pages(at::Tensor cache, std::vector<int64_t> src, std::vector<int64_t> dst,
                                               std::vector<int64_t> tokens) {
@@ -62,7 +62,8 @@ std::tuple<int64_t, int64_t> copy_cache_pages(at::Tensor cache, std::vector<int6
             "copy_cache_pages: a contiguous CUDA cache [planes, pages, block, ...] expected");
   RLB_CHECK(src.size() == dst.size() && src.size() == tokens.size(),
             "copy_cache_pages: src, dst and tokens must have one length");
-  const int64_t planes = cache.size(0), pages = cache.size(1), block = cache.size(2), none = 0;
+  const int64_t planes = cache.size(0), pages = cache.size(1), block = cache.size(2);
+  int64_t launches = 0;
   std::vector<uint8_t> written(src.empty() ? 0 : pages, 0);
   for (size_t i = 0; i < src.size(); ++i) {
     const int64_t at = i;
@@ -73,7 +74,7 @@ std::tuple<int64_t, int64_t> copy_cache_pages(at::Tensor cache, std::vector<int6
   }
   for (size_t i = 0; i < src.size(); ++i)
     if (written[src[i]]) return {4, (int64_t)i};
-  if (src.empty() || cache.numel() == 0) return {none, none};
+  if (src.empty() || cache.numel() == 0) return {0, launches};
   const c10::cuda::CUDAGuard g(cache.device());
   const long long token_bytes = cache.numel() / (planes * pages * block) * cache.element_size();
   RLB_CHECK(token_bytes < (1 << 30), "copy_cache_pages: token too large");
@@ -98,6 +99,7 @@ std::tuple<int64_t, int64_t> copy_cache_pages(at::Tensor cache, std::vector<int6
     kern<<<(unsigned)blocks, pages::kThreads, 0, stream()>>>(p, n, (uint8_t*)cache.data_ptr(), plane_bytes, page_bytes,
                                                              (int)token_bytes, (int)pieces);
     RLB_CUDA_CHECK(cudaGetLastError());
+    ++launches;
   }
-  return {none, none};
+  return {0, launches};
 }

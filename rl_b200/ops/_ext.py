@@ -50,6 +50,7 @@ _KERNELS_PER_CALL = {
     "symm_close": 0,
     "symm_view": 0,
     "moe_router_topk": 3,
+    "copy_cache_pages": 0,  # one per 640 pairs: counted by the caller
     "shared_prefix_attn": 2,
     "shared_prefix_error_flag": 0,
     "bounds_errors": 0,

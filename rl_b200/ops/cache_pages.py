@@ -13,7 +13,7 @@ from typing import Optional, Sequence, Union
 
 import torch
 
-from rl_b200.ops._ext import ext, use_native
+from rl_b200.ops._ext import add_launches, ext, use_native
 
 __all__ = ["copy_cache_pages"]
 
@@ -63,6 +63,8 @@ def copy_cache_pages(cache: torch.Tensor, src: _Ints, dst: _Ints, tokens: Option
     planes = cache.view(-1, pages, block, cache.shape[-2] * cache.shape[-1]) if cache.numel() else None
     if use_native(cache) and planes is not None:
         bad, i = ext().copy_cache_pages(planes, s, d, n)
+        if not bad:
+            add_launches(i)
     else:
         bad, i = _check_pages(s, d, n, pages, block)
     if bad == 1:

@@ -840,3 +840,12 @@ def test_rollout_decides_again_for_the_rows_that_are_left(cuda_device, heads):
         _ext.check_device_errors()
     finally:
         w.shutdown()
+
+
+def test_copy_cache_pages_launches(cuda_device):
+    cache = torch.zeros(2, 1300, 2, 1, 8, device=cuda_device)
+    for src, dst, tokens, launches in (([], [], None, 0), ([0], [1], [0], 0), ([0], [1], None, 1),
+                                       ([0] * 641, list(range(1, 642)), None, 2)):
+        before = _ext.launch_count()
+        copy_cache_pages(cache, src, dst, tokens)
+        assert _ext.launch_count() - before == launches
