@@ -138,6 +138,11 @@ BOUNDS_SITES = {1: "KV-cache slot", 2: "paged-attention block-table entry",
                 3: "expert-parallel row / rank", 4: "MoE router expert-grouped row"}
 
 
+# error words that tell of device data instead of a wait
+DATA_ERRORS = {("shared_prefix_error_flag", 1): "group starts that descend, or lengths beyond the block tables or the plan",
+               ("shared_prefix_error_flag", 2): "a block-table entry outside the cache"}
+
+
 class DeviceBoundsError(RuntimeError):
     """The bounds-checked debug build met a data-dependent index outside its
     tensor (the access was skipped)."""
@@ -145,7 +150,8 @@ class DeviceBoundsError(RuntimeError):
 
 class DeviceWaitError(RuntimeError):
     """A kernel gave up a bounded wait (a peer's flag, a copy engine's flag or a
-    pipeline barrier never arrived) and returned with its error word set."""
+    pipeline barrier never arrived), or met device data that it does not follow (``DATA_ERRORS``), and
+    returned with its error word set."""
 
 
 def check_device_errors(reset: bool = True) -> None:
@@ -163,9 +169,12 @@ def check_device_errors(reset: bool = True) -> None:
         v = int(fn(reset))
         if v:
             bad[name] = v
+    data = [f"{name}: {DATA_ERRORS[name, bad.pop(name)]}" for name in list(bad) if (name, bad[name]) in DATA_ERRORS]
     if bad:
         raise DeviceWaitError(f"device wait expired: {bad} (error word = wait site code); "
-                              "a peer rank, copy engine or pipeline stage never signalled")
+                              "a peer rank, copy engine or pipeline stage never signalled" + "".join("; " + d for d in data))
+    if data:
+        raise DeviceWaitError("device data outside its bounds: " + "; ".join(data))
     if getattr(mod, "debug_bounds_build", None) is not None and mod.debug_bounds_build():
         hits = {f: v for f, v in mod.bounds_errors(reset).items() if v}
         if hits:

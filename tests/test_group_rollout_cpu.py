@@ -273,3 +273,21 @@ def test_shared_prompts_pay_by_type_heads_and_rows(dtype, hd, nkv, rows, limit):
     tokens = -(-limit // (token * (rows - 1)))  # of one prompt for all the rows
     assert eng._shared_prefix_pays([0], [tokens] * rows, False)
     assert not eng._shared_prefix_pays([0], [tokens - 1] * rows, False)
+
+
+@pytest.mark.parametrize("words,has,lacks", [
+    ({"shared_prefix_error_flag": 1}, ["group starts"], ["wait expired"]),
+    ({"shared_prefix_error_flag": 2}, ["block-table entry"], ["wait expired"]),
+    ({"shared_prefix_error_flag": 3}, ["wait expired", "shared_prefix_error_flag"], ["block-table"]),
+    ({"shared_prefix_error_flag": 2, "gemm_error_flag": 1}, ["wait expired", "gemm_error_flag", "block-table entry"], [])])
+def test_error_words_of_device_data_are_not_called_waits(monkeypatch, words, has, lacks):
+    from types import SimpleNamespace
+
+    from rl_b200.ops import _ext
+
+    flags = {name: (lambda reset, v=words.get(name, 0): v) for name in _ext.ERROR_FLAGS}
+    monkeypatch.setattr(_ext, "has_ext", lambda: True)
+    monkeypatch.setattr(_ext, "ext", lambda: SimpleNamespace(**flags))
+    with pytest.raises(_ext.DeviceWaitError) as e:
+        _ext.check_device_errors()
+    assert all(h in str(e.value) for h in has) and not any(x in str(e.value) for x in lacks)
