@@ -508,8 +508,10 @@ __device__ __forceinline__ void drain(uint32_t bar_full, int stages, int k) {
   }
 }
 
-// factor 2^(13 - exponent) that brings a row of q of largest magnitude mx near 2^13, where f16 keeps
-// 8-bit mantissas exact over 37 binades; infinities and NaN stay, tiny rows are scaled by 2^110
+// factor 2^(13 - exponent) that brings a row of q of largest magnitude mx near 2^13, where f16 keeps bf16's
+// 8-bit mantissas exact over 31 binades (down to 2^-17, in steps of 2^-24) and loses bits gradually below; tiny
+// rows are scaled by 2^110, and one that holds an infinity or NaN not at all: what f16 cannot hold there becomes
+// infinite (such a row's scores are infinite or NaN whatever the rest)
 __device__ __forceinline__ int f16_row_exponent(float mx) {
   const int ex = (int)(__float_as_uint(mx) >> 23);
   return ex == 255 ? 140 : max(ex, 30);
@@ -794,16 +796,18 @@ struct Gen {  // shared memory of the general kernel: two CTAs on an SM
 //   16 x 16, 2048 + 2048                     80.8  71.9     111.2 111.0     120.2 126.6     207.9 218.9
 //   1 x 32, 32768 + 512                      50.2  47.9      59.8  60.7      80.7  82.0     143.7 144.5
 //
-// Against the tcgen05 kernel, the same sums:
-//   (prompts x rows, prompt + own keys)      this, bf16 128   tc    this, e4m3 128   tc   this, bf16 64   tc
-//   4 x 16, 1024 + 1024                             56.2   43.6             59.4   63.2            32.5  39.9
-//   8 x 16, 2048 + 1024                             88.7   74.2            101.1  126.3            51.1  61.2
-//   16 x 16, 2048 + 2048                           203.1  170.6            205.4  259.2           111.0 123.6
-//   1 x 32, 32768 + 512                            106.6   79.1            142.1  116.3            60.7  68.2
-// (tc with e4m3 converted its tiles to f16 in shared memory; with 64 dims it used half of its products' rows, and
-// L2 still fetched 256 bytes a key).  So bf16 caches of 128 dims go to the other kernel and the rest comes here;
-// e4m3 needs no conversion pass, since a lane's four bytes of a key are the operand words of an f16 product
-// after one conversion each.
+// Against the tcgen05 kernel, the same sums, bf16 of 128 dims, which the rule between the two sends there:
+//   (prompts x rows, prompt + own keys)         this     tc
+//   4 x 16, 1024 + 1024                         56.2   44.0
+//   8 x 16, 2048 + 1024                         88.7   74.2
+//   16 x 16, 2048 + 2048                       203.1  169.9
+//   1 x 32, 32768 + 512                        106.6   78.4
+// Earlier forms of the tcgen05 kernel for e4m3 (its tiles converted to f16 in shared memory) and for 64 dims (half of
+// its products' rows unused) took 63.2, 126.3, 259.2, 116.3 and 39.9, 61.2, 123.6, 68.2 us for the four cases, where
+// this one takes 59.4, 101.1, 205.4, 142.1 and 32.5, 51.1, 111.0, 60.7.  Both were measured while L2 fetched 256 bytes
+// for a key of 128, which has cost this kernel up to a fifth: the rule is settled for bf16 of 128 dims, and for the
+// rest it says what is built.  One prompt with an e4m3 cache was faster there even so.  Here e4m3 needs no conversion
+// pass: a lane's four bytes of a key are the operand words of an f16 product after one conversion each.
 template <int HD, bool F8>
 __global__ void __launch_bounds__(160, 2)
 shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -947,11 +951,12 @@ shared_prefix_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_c
 // the rate of a plain copy):
 //   16 prompts of up to 2048 keys x 8-16 rows with up to 2048 own keys   160 us, 5.7 TB/s (floor 139 us)
 //   4 prompts of up to 1024 keys x 8-16 rows with up to 1024 own keys     34 us, 3.6 TB/s (floor 19 us)
-//   1 prompt of 32768 keys x 32 rows                                      63 us, 2.7 TB/s (floor 26 us)
-// The first is bound by HBM.  Where prompts dominate, a tile costs about 3000 cycles of a softmax group at 64
-// columns (issue and latency of 64 exponentials a thread) against the 2770 cycles that HBM needs for its bytes
-// and half of that where two units read the same keys; short units add about a tile's time each for their
-// query rows, first scores and output.
+//   1 prompt of 32768 keys x 32 rows                                      64 us, 2.7 TB/s (floor 26 us)
+// The first is bound by HBM.  In the third a CTA has about 28 prefix and 4 suffix tiles: some 3700 cycles a tile,
+// where HBM needs 1390 for its bytes (two units read the same keys), the exponentials of 64 columns about 512, and
+// two softmax groups of some 3000 cycles a tile, in turns, 1500.  What fills the rest has not been found: the groups
+// may not overlap, or the two units of a key drift apart (28 % L2 hits, of 50 % possible).  Short units add about a
+// tile's time each for their query rows, first scores and output.
 //
 // Tried and not kept: the two products of a query row on the M side (128 rows a unit; a suffix then costs as
 // much as a prefix), mma.sync for the suffix beside it (16-key steps are 300 instructions of latency), one

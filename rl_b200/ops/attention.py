@@ -284,10 +284,14 @@ def shared_prefix_decode_attention(q, k_cache, v_cache, block_tables, seq_lens, 
     alone; a row of length 0 gives zeros and bounds no group.  A prefix longer than a row of its
     group is shared up to that row's length.
 
+    On a GPU the softmax weights are rounded to bf16, or f16 with an e4m3 cache, for the product with V, and
+    sums are taken in another order than row by row: results agree within those roundings, not bit for bit.
+
     ``plan`` (:func:`shared_prefix_plan` of the same lengths) saves planning once per layer; it is
     followed whatever the lengths are now.  Lengths and tables are device data: table entries
-    outside the cache, lengths beyond the tables and group starts that descend are not followed but
-    reported by :func:`rl_b200.ops._ext.check_device_errors`.
+    outside the cache, lengths beyond the tables (or beyond what a plan numbers: at least 64 x 2^30 keys over
+    KV heads x (2 rows + groups)) and group starts that descend are not followed but reported by
+    :func:`rl_b200.ops._ext.check_device_errors`.
     """
     _check_groups(seq_lens, group_starts, prefix_lens)
     B = q.shape[0] if q.dim() == 3 else -1
